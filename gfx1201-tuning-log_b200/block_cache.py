@@ -1,0 +1,134 @@
+"""A paged fp8 cache with a scale per block and kv head: append and attention.
+
+`append` rotates the new tokens' q and k and writes k and v into the cache;
+`attention` runs causal attention of a varlen batch over it, from one query
+token a sequence to whole prompts, with an optional sliding window and first
+tokens that stay visible.  The kernels are csrc/block_append.cu and
+csrc/block_attn.cu, through b200kv_block_append and b200kv_block_attn.
+
+The cache of a layer is k_cache / v_cache, float8_e4m3fn [NB, BS, HKV, 128] (any
+strides with unit innermost; BS 16, 32, 64 or 128), and k_scales / v_scales,
+float32 [NB, HKV]: a code stands for code * scale.  Sequence s keeps token p at
+block block_table[s, p // BS], slot p % BS.  Neither call reads the host's copy
+of a length, so both can be captured in CUDA graphs.
+"""
+import ctypes
+
+import torch
+
+from _b200kv import BlockAttnArgs, BlockCacheDesc, check, lib
+
+HEAD_DIM = 128
+_FP8 = torch.float8_e4m3fn
+
+
+def _describe(k_cache, v_cache, k_scales, v_scales, block_table):
+    if k_cache.dtype != _FP8 or v_cache.dtype != _FP8:
+        raise TypeError("k_cache and v_cache must be float8_e4m3fn")
+    if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
+        raise TypeError("k_scales and v_scales must be float32")
+    if block_table.dtype != torch.int32:
+        raise TypeError("block_table must be int32")
+    nb, bs, hkv, d = k_cache.shape
+    if v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache and v_cache shapes differ")
+    if k_scales.shape != (nb, hkv) or v_scales.shape != (nb, hkv):
+        raise ValueError(f"k_scales and v_scales must be [{nb}, {hkv}]")
+    sk, sv, bt = k_cache.stride(), v_cache.stride(), block_table.stride()
+    if sk[3] != 1 or sv[3] != 1 or bt[1] != 1:
+        raise ValueError("k_cache, v_cache and block_table must have unit innermost stride")
+    seqs, blocks = block_table.shape
+    ks, vs = k_scales.stride(), v_scales.stride()
+    return BlockCacheDesc(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                          block_table.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], ks[0], ks[1], vs[0],
+                          vs[1], bt[0], nb, bs, hkv, d, blocks, seqs)
+
+
+def _batch(cu_seqlens, seq_lens, seqs):
+    if cu_seqlens.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise TypeError("cu_seqlens and seq_lens must be int32")
+    if cu_seqlens.shape != (seqs + 1,) or seq_lens.shape != (seqs,):
+        raise ValueError(f"cu_seqlens must be [{seqs + 1}] and seq_lens [{seqs}], as block_table has rows")
+    if not (cu_seqlens.is_contiguous() and seq_lens.is_contiguous()):
+        raise ValueError("cu_seqlens and seq_lens must be contiguous")
+
+
+def append(qkv, cos_sin, k_cache, v_cache, k_scales, v_scales, cu_seqlens, seq_lens, block_table, q_out=None):
+    """Rotate and append the batch's new tokens; returns the rotated q [T, HQ, 128].
+
+    qkv bf16 [T, (HQ + 2 HKV) 128], the fused projection (rows may be strided);
+    cos_sin float32 [max_pos, 128] (decoder.rope_table); rows cu_seqlens[s] ..
+    cu_seqlens[s+1] - 1 are the last tokens of sequence s, which has seq_lens[s]
+    tokens with them.  q_out (bf16 [T, HQ, 128]) defaults to the q columns of qkv,
+    rotated in place.  A block's scale is the smallest power of two that fits its
+    values (x / scale within e4m3's 448); a block that outgrows it has its earlier
+    codes rounded again.  Two sequences may not append to one block.
+    """
+    if qkv.dtype != torch.bfloat16:
+        raise TypeError("qkv must be bfloat16")
+    if cos_sin.dtype != torch.float32:
+        raise TypeError("cos_sin must be float32")
+    desc = _describe(k_cache, v_cache, k_scales, v_scales, block_table)
+    _batch(cu_seqlens, seq_lens, desc.num_seqs)
+    tokens, width = qkv.shape
+    hq = width // HEAD_DIM - 2 * desc.num_kv_heads
+    if width % HEAD_DIM or hq <= 0 or hq % desc.num_kv_heads:
+        raise ValueError(f"qkv rows of {width} are not [q | k | v] heads of {HEAD_DIM} over {desc.num_kv_heads} kv heads")
+    if cos_sin.dim() != 2 or cos_sin.shape[1] != HEAD_DIM or not cos_sin.is_contiguous() or qkv.stride(1) != 1:
+        raise ValueError("cos_sin must be contiguous [max_pos, 128] and qkv rows contiguous")
+    if q_out is None:
+        q_out = qkv[:, :hq * HEAD_DIM].unflatten(1, (hq, HEAD_DIM))
+    elif q_out.dtype != torch.bfloat16:
+        raise TypeError("q_out must be bfloat16")
+    if q_out.shape != (tokens, hq, HEAD_DIM) or q_out.stride(2) != 1:
+        raise ValueError(f"q_out must be [{tokens}, {hq}, {HEAD_DIM}] with unit innermost stride")
+    check(lib.b200kv_block_append(
+        ctypes.byref(desc), qkv.data_ptr(), qkv.stride(0), cos_sin.data_ptr(), cos_sin.shape[0], q_out.data_ptr(),
+        q_out.stride(0), q_out.stride(1), cu_seqlens.data_ptr(), seq_lens.data_ptr(), tokens, hq,
+        torch.cuda.current_stream(qkv.device).cuda_stream), "b200kv_block_append")
+    return q_out
+
+
+class Workspace:
+    """Scratch of `attention` for batches of up to num_seqs sequences over
+    num_kv_heads heads: partial results of contexts split over several CTAs and
+    the counters that join them.  Calls that share one are ordered on one stream
+    (graph replays included)."""
+
+    def __init__(self, device, num_seqs, num_kv_heads):
+        self.num_seqs, self.num_kv_heads = num_seqs, num_kv_heads
+        self.buffer = torch.zeros(lib.b200kv_block_attn_workspace_bytes(num_seqs, num_kv_heads), dtype=torch.uint8,
+                                  device=device)
+
+
+def attention(q, k_cache, v_cache, k_scales, v_scales, out, cu_seqlens_q, seq_lens, block_table, sm_scale, max_qlen,
+              max_seq_len=0, window=0, sinks=0, workspace=None):
+    """Causal attention of the batch's queries over the cache into out.
+
+    q, out bf16 [T, HQ, 128] (unit innermost stride), HQ / HKV at most 16.  Query
+    i of sequence s (row cu_seqlens_q[s] + i) is at position p = seq_lens[s] -
+    qlen + i and sees keys j <= p; with window > 0 those with j > p - window or
+    j < sinks.  A query that sees no key gives zeros.  max_qlen and max_seq_len
+    (0: what block_table holds) bound the batch's query counts and lengths.
+    workspace: a Workspace, or None for one made for this call.
+    """
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+        raise TypeError("q and out must be bfloat16")
+    desc = _describe(k_cache, v_cache, k_scales, v_scales, block_table)
+    _batch(cu_seqlens_q, seq_lens, desc.num_seqs)
+    if q.dim() != 3 or q.shape[2] != HEAD_DIM or out.shape != q.shape:
+        raise ValueError(f"q and out must be [tokens, heads, {HEAD_DIM}]")
+    sq, so = q.stride(), out.stride()
+    if sq[2] != 1 or so[2] != 1:
+        raise ValueError("q and out must have unit innermost stride")
+    if workspace is None:
+        workspace = Workspace(q.device, desc.num_seqs, desc.num_kv_heads)
+    elif workspace.num_seqs < desc.num_seqs or workspace.num_kv_heads < desc.num_kv_heads:
+        raise ValueError("workspace is for fewer sequences or kv heads")
+    ws = workspace.buffer
+    args = BlockAttnArgs(q.data_ptr(), out.data_ptr(), cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), ws.data_ptr(),
+                         ws.numel(), sq[0], sq[1], so[0], so[1], sm_scale, q.shape[0], max_qlen,
+                         max_seq_len or desc.max_blocks * desc.block_size, q.shape[1], window, sinks, 0)
+    check(lib.b200kv_block_attn(ctypes.byref(desc), ctypes.byref(args),
+                                torch.cuda.current_stream(q.device).cuda_stream), "b200kv_block_attn")
+    return out

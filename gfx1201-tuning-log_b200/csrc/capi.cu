@@ -122,6 +122,16 @@ int prefill_attn_launch(const void* q, int64_t q_st, int64_t q_sh, const void* k
                         int block_size, int num_blocks, int kv_dtype, int only_multi, void* stream,
                         int total_q);
 
+int block_append_launch(const b200kv_block_cache* c, const void* qkv, int64_t qkv_st, const float* cos_sin,
+                        int max_pos, void* q_out, int64_t q_st, int64_t q_sh, const int32_t* cu,
+                        const int32_t* lens, int num_tokens, int hq, void* stream);
+size_t block_attn_workspace_bytes(int num_seqs, int num_kv_heads);
+int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args* a, void* stream);
+int spec_verify_launch(const void* logits, int64_t ld, int half, const int64_t* tokens, const int32_t* cu,
+                       const float* uniforms, const float* noise, int64_t noise_ld, const float* temperature,
+                       const float* draft, int64_t draft_ld, int64_t* out, int32_t* accepted, int num_seqs,
+                       int num_rows, int vocab, void* stream);
+
 void set_last_error(int e) { t_last_error = e; }
 
 }  // namespace b200kv
@@ -335,6 +345,31 @@ int b200kv_kv_write(const void* key, int64_t key_stride_tok, int64_t key_stride_
 }
 
 }  // extern "C"
+
+// ---- block-scaled cache and draft verification --------------------------------------
+extern "C" int b200kv_block_append(const b200kv_block_cache* cache, const void* qkv, int64_t qkv_stride,
+                                   const float* cos_sin, int max_pos, void* q_out, int64_t q_stride_tok,
+                                   int64_t q_stride_head, const int32_t* cu_seqlens, const int32_t* seq_lens,
+                                   int num_tokens, int num_q_heads, void* stream) {
+  return b200kv::block_append_launch(cache, qkv, qkv_stride, cos_sin, max_pos, q_out, q_stride_tok, q_stride_head,
+                                     cu_seqlens, seq_lens, num_tokens, num_q_heads, stream);
+}
+extern "C" size_t b200kv_block_attn_workspace_bytes(int num_seqs, int num_kv_heads) {
+  return b200kv::block_attn_workspace_bytes(num_seqs, num_kv_heads);
+}
+extern "C" int b200kv_block_attn(const b200kv_block_cache* cache, const b200kv_block_attn_args* args,
+                                 void* stream) {
+  return b200kv::block_attn_launch(cache, args, stream);
+}
+extern "C" int b200kv_spec_verify(const void* logits, int64_t ld, int half, const int64_t* tokens,
+                                  const int32_t* cu_rows, const float* uniforms, const float* noise,
+                                  int64_t noise_ld, const float* temperature, const float* draft_probs,
+                                  int64_t draft_ld, int64_t* out_tokens, int32_t* num_accepted, int num_seqs,
+                                  int num_rows, int vocab, void* stream) {
+  return b200kv::spec_verify_launch(logits, ld, half, tokens, cu_rows, uniforms, noise, noise_ld, temperature,
+                                    draft_probs, draft_ld, out_tokens, num_accepted, num_seqs, num_rows, vocab,
+                                    stream);
+}
 
 // ---- tensor-parallel allreduce over peer memory ------------------------------------
 extern "C" size_t b200kv_comm_buffer_bytes(void) { return b200kv::comm_buffer_bytes(); }

@@ -424,6 +424,103 @@ int b200kv_rope_kv_write(void* qkv, int64_t qkv_stride_tok, const int32_t* posit
                          int head_dim, int block_size, int kv_dtype, void* stream);
 int b200kv_swiglu(const void* gate_up, void* act, int rows, int inter, void* stream);
 
+/* ---- block-scaled fp8 cache: append, attention ------------------------------------
+ *
+ * A paged e4m3 cache with one fp32 scale for each (block, kv head) of K and of
+ * V: the value of a code is code * scale[block, kv head].  No counterpart in the
+ * reference, whose cache has one scale per tensor.
+ *
+ *   k / v         e4m3 [num_blocks, block_size, num_kv_heads, 128], strides
+ *                 (s*0, s*1, s*2, 1), multiples of 16, 16-byte aligned
+ *   k/v_scales    fp32 [num_blocks, num_kv_heads], strides (ks*, vs*), >= 0
+ *   block_table   int32 [num_seqs, >= max_blocks], row stride bt_stride
+ *   block_size    16, 32, 64 or 128; head_dim 128
+ *
+ * A block id outside [0, num_blocks) reads as zeros and is never written.
+ */
+typedef struct b200kv_block_cache {
+  void* k;
+  void* v;
+  float* k_scales;
+  float* v_scales;
+  const int32_t* block_table;
+  int64_t sk0, sk1, sk2, sv0, sv1, sv2;
+  int64_t ks0, ks1, vs0, vs1;
+  int64_t bt_stride;
+  int32_t num_blocks, block_size, num_kv_heads, head_dim;
+  int32_t max_blocks, num_seqs;
+} b200kv_block_cache;
+
+/* b200kv_block_append: the new tokens of a batch, rotated and written.  Rows
+ * cu_seqlens[s] .. cu_seqlens[s+1]-1 of qkv (bf16, [q heads | k heads | v heads]
+ * of 128, row stride qkv_stride) are the last tokens of sequence s, whose length
+ * with them is seq_lens[s].  Per token at position p:
+ *   q_out[t, h, :] = bf16(rot(q, p)), k and v codes at block_table[s, p / block_size].
+ * rot: neox halves in fp32, products rounded before the sum, as
+ * b200kv_rope_kv_write; cos_sin fp32 [max_pos][128], positions clamped to it.
+ * A block's scale becomes the smallest power of two s with amax <= 448 s over the
+ * call's finite new values of that block and head (exponent in [-64, 100]; 2^-64
+ * when all are zero).  Where the block holds earlier tokens of the sequence (its
+ * first new token is not at the block's start) the scale never shrinks, and when
+ * it grows the earlier tokens' codes are rounded again: e4m3(code * old / new).
+ * Codes are e4m3(x / s), saturating, from the unrounded fp32 value.
+ * q_out may be the q columns of qkv.  Two sequences may not append to one block.
+ * A position outside the table or a block id outside the cache is skipped and
+ * records B200KV_DEV_INDEX_RANGE (its q is rotated all the same). */
+int b200kv_block_append(const b200kv_block_cache* cache, const void* qkv, int64_t qkv_stride,
+                        const float* cos_sin, int max_pos, void* q_out, int64_t q_stride_tok,
+                        int64_t q_stride_head, const int32_t* cu_seqlens, const int32_t* seq_lens,
+                        int num_tokens, int num_q_heads, void* stream);
+
+/* b200kv_block_attn: causal attention of a varlen batch over the cache.  Query i
+ * of sequence s (row cu_seqlens_q[s] + i) is at position p = seq_lens[s] - qlen + i
+ * and sees the keys j <= p with window == 0, j > p - window or j < sinks:
+ *   out[row, h, :] = sum_j softmax_j(sm_scale q . K[j]) V[j]      (bf16)
+ * A query that sees nothing (p < 0) gives zeros.  GQA 1 to 16.
+ *   num_tokens    rows of q; max_qlen, max_seq_len  upper bounds over the batch
+ *   workspace     b200kv_block_attn_workspace_bytes bytes, 256-byte aligned, zeroed
+ *                 once before its first use (every call leaves its counters at
+ *                 zero); calls that share one are ordered on one stream. */
+typedef struct b200kv_block_attn_args {
+  const void* q;
+  void* out;
+  const int32_t* cu_seqlens_q;
+  const int32_t* seq_lens;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t q_stride_tok, q_stride_head, out_stride_tok, out_stride_head;
+  float sm_scale;
+  int32_t num_tokens, max_qlen, max_seq_len, num_q_heads;
+  int32_t window, sinks;
+  int32_t reserved;   /* 0 */
+} b200kv_block_attn_args;
+size_t b200kv_block_attn_workspace_bytes(int num_seqs, int num_kv_heads);
+int b200kv_block_attn(const b200kv_block_cache* cache, const b200kv_block_attn_args* args, void* stream);
+
+/* ---- verification of drafted tokens -------------------------------------------------
+ *
+ * Rows cu_rows[s] .. cu_rows[s+1]-1 of logits (fp32, or bf16 when half != 0; row
+ * stride ld) are the target's logits of sequence s after its last token and each
+ * of its drafts; tokens (int64, one per row) are the ids fed to those rows, so
+ * tokens[r+1] is the draft that row r verifies.  With p_r = softmax(logits[r] /
+ * temperature[s]) (temperature 0: one at the lowest index of the maximum) and
+ * q_r = draft_probs[r] (fp32, row stride draft_ld; NULL: one at the draft):
+ *   row r's draft d is taken while uniforms[r] * q_r(d) < p_r(d);
+ *   the first row that does not take its draft emits argmax_v max(p_r - q_r, 0)(v) /
+ *   noise[s, v] (p_r / noise where no v has p_r > q_r), the last row, when all
+ *   are taken, argmax_v p_r(v) / noise[s, v]; ties to the lowest index.
+ * With uniforms ~ U[0, 1) and noise ~ Exp(1) (fp32 [num_seqs, vocab], row stride
+ * noise_ld, > 0) the emitted tokens are distributed as the target's.
+ *   out_tokens    int64, one per row: the taken drafts, the emitted token, then -1
+ *   num_accepted  int32 [num_seqs]: drafts taken
+ * A logit of NaN counts as -inf, infinities as the largest finite value; a row of
+ * -inf takes no draft and emits token 0.  A draft outside [0, vocab) is not
+ * taken.  temperature NULL: 1.  No counterpart in the reference. */
+int b200kv_spec_verify(const void* logits, int64_t ld, int half, const int64_t* tokens, const int32_t* cu_rows,
+                       const float* uniforms, const float* noise, int64_t noise_ld, const float* temperature,
+                       const float* draft_probs, int64_t draft_ld, int64_t* out_tokens, int32_t* num_accepted,
+                       int num_seqs, int num_rows, int vocab, void* stream);
+
 /* ---- Tensor-parallel allreduce over peer memory ---------------------------------
  *
  * Sum of a bf16 vector of n elements (n % 8 == 0, n <= 32768: one [M <= 8, 4096]
