@@ -127,7 +127,6 @@ __global__ void __launch_bounds__(NW * 32) block_append_kernel(const AppendParam
   const int begin = total - qlen;
   const int page = (begin >> p.shift) + (item - first_item(row_s - c0, seq, p.shift));
   if (qlen <= 0 || page > ((total - 1) >> p.shift)) return;
-  const int bs = 1 << p.shift;
   const int lo = max(begin, page << p.shift), hi = min(total, (page + 1) << p.shift);
   const int nt = hi - lo, row0 = row_s + (lo - begin);
   const int kept = lo - (page << p.shift);  // earlier tokens of this block

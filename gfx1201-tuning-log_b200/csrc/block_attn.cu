@@ -11,6 +11,8 @@
 
 #include "b200kv.h"
 #include "b200kv_common.cuh"
+#include "block_attn.cuh"
+#include "tma.cuh"
 
 namespace b200kv {
 
@@ -19,31 +21,13 @@ int block_cache_check(const b200kv_block_cache* c);
 namespace {
 
 constexpr int kHead = 128;
-constexpr int kMaxGroup = 16;
-
-struct PlainAttnParams {
-  const __nv_bfloat16* q;
-  __nv_bfloat16* out;
-  int64_t q_st, q_sh, o_st, o_sh;
-  const int32_t* cu;
-  const int32_t* lens;
-  const int32_t* bt;
-  int64_t bt_stride;
-  const uint8_t* kc;
-  const uint8_t* vc;
-  const float* ks;
-  const float* vs;
-  int64_t sk0, sk1, sk2, sv0, sv1, sv2, ks0, ks1, vs0, vs1;
-  float sm_scale;
-  int num_seqs, group, shift, num_blocks, max_blocks, window, sinks;
-};
 
 __device__ __forceinline__ float e4m3(uint8_t b) {
   const __half_raw h = __nv_cvt_fp8_to_halfraw(b, __NV_E4M3);
   return __half2float(*reinterpret_cast<const __half*>(&h));
 }
 
-__global__ void __launch_bounds__(kHead) block_attn_plain_kernel(const PlainAttnParams p) {
+__global__ void __launch_bounds__(kHead) block_attn_plain_kernel(const BlockAttnParams p) {
   __shared__ float s_q[kMaxGroup][kHead], s_p[kMaxGroup][kHead], s_red[kHead / 32][kMaxGroup];
   __shared__ float s_vs[kHead];
   __shared__ int64_t s_v[kHead];
@@ -53,6 +37,7 @@ __global__ void __launch_bounds__(kHead) block_attn_plain_kernel(const PlainAttn
   int seq = 0;
   while (seq + 1 < p.num_seqs && p.cu[seq + 1] <= row) ++seq;
   if (row < p.cu[seq] || row >= p.cu[seq + 1]) return;
+  if ((p.cu[seq + 1] - p.cu[seq]) * G <= kMaxRows) return;  // the few-query kernel's
   const int pos = p.lens[seq] - (p.cu[seq + 1] - row);
   for (int g = 0; g < G; ++g)
     s_q[g][tid] = __bfloat162float(p.q[(int64_t)row * p.q_st + (int64_t)(kh * G + g) * p.q_sh + tid]);
@@ -132,8 +117,11 @@ __global__ void __launch_bounds__(kHead) block_attn_plain_kernel(const PlainAttn
 
 }  // namespace
 
+// counters, then the partials
 size_t block_attn_workspace_bytes(int num_seqs, int num_kv_heads) {
-  return num_seqs > 0 && num_kv_heads > 0 ? 256 : 0;
+  if (num_seqs <= 0 || num_kv_heads <= 0) return 0;
+  return align_up((size_t)num_seqs * num_kv_heads * sizeof(int), 256) +
+         (size_t)2 * kMaxCtas * kMaxRows * (kHead + 2) * sizeof(float);
 }
 
 int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args* a, void* stream) {
@@ -152,7 +140,7 @@ int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args*
   if (reinterpret_cast<uintptr_t>(a->workspace) & 255) return B200KV_ERR_MISALIGNED;
   if (sm_major_current_device() < 10) return B200KV_ERR_NO_DEVICE;
   if (a->num_tokens == 0) return B200KV_OK;
-  PlainAttnParams p;
+  BlockAttnParams p;
   p.q = static_cast<const __nv_bfloat16*>(a->q);
   p.out = static_cast<__nv_bfloat16*>(a->out);
   p.q_st = a->q_stride_tok; p.q_sh = a->q_stride_head;
@@ -173,10 +161,25 @@ int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args*
   p.group = a->num_q_heads / c->num_kv_heads;
   p.shift = __builtin_ctz((unsigned)c->block_size);
   p.num_blocks = c->num_blocks;
-  p.max_blocks = c->max_blocks;
+  p.max_blocks = c->max_blocks < (0x7fffffff >> p.shift) ? c->max_blocks : 0x7fffffff >> p.shift;
   p.window = a->window;
   p.sinks = a->sinks;
-  block_attn_plain_kernel<<<dim3(a->num_tokens, c->num_kv_heads), kHead, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  p.hkv = c->num_kv_heads;
+  p.counters = static_cast<int*>(a->workspace);
+  p.partials = reinterpret_cast<float*>(static_cast<char*>(a->workspace) +
+                                        align_up((size_t)c->num_seqs * c->num_kv_heads * sizeof(int), 256));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  CUtensorMap km, vm;
+  if (!encode_paged_kv(&km, c->k, kHead, (uint32_t)c->num_kv_heads, (uint32_t)c->block_size, (uint64_t)c->num_blocks,
+                       (uint64_t)c->sk2, (uint64_t)c->sk1, (uint64_t)c->sk0) ||
+      !encode_paged_kv(&vm, c->v, kHead, (uint32_t)c->num_kv_heads, (uint32_t)c->block_size, (uint64_t)c->num_blocks,
+                       (uint64_t)c->sv2, (uint64_t)c->sv1, (uint64_t)c->sv0))
+    return B200KV_ERR_UNSUPPORTED;
+  const int64_t rows = (int64_t)a->max_qlen * p.group;
+  if (block_decode_launch(km, vm, p, rows < kMaxRows ? (int)rows : kMaxRows, st) != cudaSuccess)
+    return B200KV_ERR_LAUNCH;
+  if (rows <= kMaxRows) return B200KV_OK;
+  block_attn_plain_kernel<<<dim3(a->num_tokens, c->num_kv_heads), kHead, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? B200KV_OK : B200KV_ERR_LAUNCH;
 }
 

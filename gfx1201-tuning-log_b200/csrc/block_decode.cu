@@ -1,0 +1,688 @@
+// Attention of a few query tokens a sequence over a block-scaled fp8 paged cache
+// (sm_100a): decoding and verification steps, at most kMaxRows (query token, head)
+// rows per kv head.
+//
+// The keys are the long side, so they are the M = 128 side of both products:
+//   S^T [128 keys x rows]  = K Q^T,   O^T [128 dims x rows] += V^T P^T,
+// kind::f8f6f4 MMAs on the e4m3 tiles as the TMA lands them (K is K-major, V^T
+// MN-major, no conversion).  Q and P enter as two e4m3 terms, hi and 16 lo, in
+// columns of their own (N = 2 rows), added after the product: 8 significant bits
+// each.  One 128-key tile (32 KB of K and V) costs eight MMAs, whatever the rows.
+//
+// Block scales.  With a key's scales ks and vs,
+//   x = sm_scale log2(e) ks (q . k) + log2(vs),   P = 2^(x - m),  m >= max x (lazily)
+// weights the V codes directly, and the softmax sum adds P / vs.  The reference m
+// so follows the size of the contributions p vs, which keeps P in e4m3's range
+// whatever the blocks' scales; vs is taken in [2^-80, 2^80].
+//
+// One CTA per SM walks a contiguous range of the batch's tiles, ordered by
+// (sequence, kv head, tile) and cut into equal shares on the device from the
+// lengths, so a ragged batch keeps every SM equally busy and the K/V ring never
+// drains between items.  Shares that cut an item leave (o, m, l) in the workspace;
+// the last CTA of the item to finish (a counter, back at zero afterwards) joins
+// them in order, so the sum does not depend on who is last.
+//
+// Roles: 8 softmax warps in two groups that take alternate tiles (own S, O, P and
+// running state each, joined at the item's end), a TMA warp, an MMA warp.  A
+// softmax thread is one key: it reads its row of S^T, the group finds each row's
+// maximum (a warp maximum and an exchange through shared memory), and P goes to
+// shared memory as the K-major B operand.  Keys no query sees have their V rows
+// zeroed, so stale or non-finite codes never reach an output.
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "b200kv.h"
+#include "b200kv_common.cuh"
+#include "block_attn.cuh"
+#include "fp8_terms.cuh"
+#include "tcgen05.cuh"
+#include "tma.cuh"
+
+namespace b200kv {
+namespace {
+
+constexpr int kHead = 128;
+constexpr int kTile = 128;                  // keys per tile
+constexpr int kHalf = kTile * kHead;        // K (or V) bytes of a tile
+constexpr int kGroupWarps = 4;
+constexpr int kSoftWarps = 2 * kGroupWarps;
+constexpr int kThreads = (kSoftWarps + 2) * 32;
+constexpr int kMaxPages = 8;                // pages per tile
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 4.f;                // the reference moves when a maximum exceeds it by 2^4
+constexpr float kOff = 4.f;                 // P is formed times 2^4 (at most 2^8)
+constexpr float kLo = 16.f;                 // the second terms carry 16 times the remainder
+constexpr float kMinScale = 8.2718061e-25f; // 2^-80
+constexpr float kMaxScale = 1.2089258e24f;  // 2^80
+
+template <int R>
+struct Shape {
+  static constexpr int kN = 2 * R;          // columns of S^T and O^T: hi rows, lo rows
+  static constexpr int kStages = R >= 64 ? 4 : R == 32 ? 5 : 6;
+  static constexpr int kOperand = kN * 128; // bytes of Q or P
+  static constexpr int kOffQ = kStages * 2 * kHalf;  // [segment parity]
+  static constexpr int kOffP = kOffQ + 2 * kOperand; // [group]; the groups' join at a segment's end
+  static constexpr int kBytes = kOffP + 2 * kOperand;
+  static constexpr int kChunk = R < 16 ? R : 16;     // rows handled together
+  static constexpr int kLook = R >= 64 ? 2 : 4;      // score tiles in tensor memory
+  static constexpr uint32_t kTmem = R == 8 ? 128 : R == 16 ? 256 : 512;  // kLook S + 2 O tiles of N columns
+  static_assert((kLook + 2) * kN <= (int)kTmem && kStages > kLook, "tensor memory; a stage free to load into");
+};
+
+template <int R>
+struct Shared {
+  uint64_t kv_full[Shape<R>::kStages], kv_empty[Shape<R>::kStages];
+  uint64_t q_full[2], s_full[Shape<R>::kLook], p_full[2], pv_done[2];
+  uint32_t tmem;
+  float scale[Shape<R>::kStages][2][kMaxPages];      // ks, vs of a tile's pages
+  alignas(16) float factor[2][R];                    // [segment parity] score factor of a row
+  alignas(16) int pos[2][R];                         // and its position
+  alignas(16) float part_max[2][2][kGroupWarps][R];  // [group][tile parity][warp]
+  alignas(16) float ref[2][2][R];                    // [group][tile parity] the reference m
+  alignas(16) float fin_m[2][R], fin_l[2][kGroupWarps][R];
+  int first_seq, first_prefix, last;
+  int warp_sum[kSoftWarps + 2];
+};
+
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+// 4 bytes to shared memory (zeros when !ok, src unread), counted by async_arrive of
+// the same thread
+__device__ __forceinline__ void async_word(void* dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// The tiles of one sequence that any of its queries sees.
+struct Span {
+  int qlen, total, kv_end, q0, row0;
+  int sink_tiles, low_tile, tiles;  // tiles 0 .. sink_tiles - 1, then low_tile ..
+  __device__ __forceinline__ int tile(int j) const { return j < sink_tiles ? j : low_tile + j - sink_tiles; }
+};
+__device__ __forceinline__ Span span_of(const BlockAttnParams& p, int seq, int max_rows) {
+  Span s;
+  s.row0 = p.cu[seq];
+  s.qlen = p.cu[seq + 1] - s.row0;
+  s.total = p.lens[seq];
+  s.q0 = s.total - s.qlen;
+  s.kv_end = min(s.total, p.max_blocks << p.shift);
+  s.tiles = s.sink_tiles = s.low_tile = 0;
+  if (s.qlen <= 0 || s.qlen > max_rows || s.qlen * p.group > max_rows || s.kv_end <= 0) return s;
+  const int high = (s.kv_end + kTile - 1) / kTile;
+  if (p.window > 0) {
+    s.low_tile = min(max(0, s.q0 - p.window + 1) / kTile, high);
+    s.sink_tiles = min(min(p.sinks, s.kv_end) + kTile - 1, s.kv_end + kTile - 1) / kTile;
+    s.sink_tiles = min(s.sink_tiles, s.low_tile);
+  }
+  s.tiles = s.sink_tiles + high - s.low_tile;
+  return s;
+}
+
+// A CTA's share, segment by segment (a segment: consecutive tiles of one item).
+struct Walk {
+  const BlockAttnParams& p;
+  int max_rows;
+  Span s;
+  int seq, kh, off, left;
+  int64_t item;  // index of the item's first tile among the batch's
+  __device__ Walk(const BlockAttnParams& p_, int max_rows_, int seq_, int prefix, int64_t begin, int count)
+      : p(p_), max_rows(max_rows_), seq(seq_), left(count) {
+    s = span_of(p, seq, max_rows);
+    const int rel = (int)(begin - (int64_t)prefix * p.hkv);
+    kh = rel / s.tiles;
+    off = rel - kh * s.tiles;
+    item = begin - off;
+  }
+  __device__ __forceinline__ int count() const { return min(s.tiles - off, left); }
+  __device__ __forceinline__ void next() {
+    left -= count();
+    if (left <= 0) return;
+    item += s.tiles;
+    off = 0;
+    if (++kh == p.hkv) {
+      kh = 0;
+      do {
+        s = span_of(p, ++seq, max_rows);
+      } while (s.tiles == 0 && seq + 1 < p.num_seqs);
+    }
+  }
+};
+
+__device__ __forceinline__ int64_t share_begin(int64_t cta, int64_t total, int64_t ctas) { return cta * total / ctas; }
+__device__ __forceinline__ int share_owner(int64_t tile, int64_t total, int64_t ctas) {
+  return (int)(((tile + 1) * ctas - 1) / total);
+}
+
+template <int R>
+__global__ void __launch_bounds__(kThreads, 1)
+    block_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                        const BlockAttnParams p) {
+  using SH = Shape<R>;
+  constexpr int N = SH::kN, NS = SH::kStages, CH = SH::kChunk, LK = SH::kLook;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ Shared<R> S;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  if (tid == 0) {
+    griddep_launch_dependents();
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&S.kv_full[s], 1 + 32);  // the bytes of the tile, and each producer lane's scales
+      mbar_init(&S.kv_empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&S.q_full[b], kSoftWarps);
+      mbar_init(&S.p_full[b], kGroupWarps);
+      mbar_init(&S.pv_done[b], 1);
+    }
+    for (int b = 0; b < LK; ++b) mbar_init(&S.s_full[b], 1);
+    fence_mbar_init();
+  }
+  if (warp == kSoftWarps + 1) tc::tmem_alloc(&S.tmem, SH::kTmem);
+  griddep_wait();  // lengths, tables and q may be the previous kernel's
+
+  // ---- this CTA's share: an inclusive scan of the sequences' tile counts -------------
+  const int per = (p.num_seqs + kThreads - 1) / kThreads;
+  const int s_lo = min(p.num_seqs, tid * per), s_hi = min(p.num_seqs, s_lo + per);
+  int mine = 0;
+  for (int s = s_lo; s < s_hi; ++s) mine += span_of(p, s, R).tiles;
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) S.warp_sum[warp] = incl;
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  int before = 0, tiles = 0;
+#pragma unroll
+  for (int w = 0; w < kSoftWarps + 2; ++w) {
+    if (w < warp) before += S.warp_sum[w];
+    tiles += S.warp_sum[w];
+  }
+  const int64_t total = (int64_t)tiles * p.hkv;
+  const int64_t ctas = min((int64_t)gridDim.x, total);
+  const bool busy = blockIdx.x < ctas;
+  const int64_t begin = busy ? share_begin(blockIdx.x, total, ctas) : 0;
+  const int count = busy ? (int)(share_begin(blockIdx.x + 1, total, ctas) - begin) : 0;
+  if (busy) {
+    int at = before + incl - mine;  // tiles of the sequences before this thread's
+    if (begin >= (int64_t)at * p.hkv && begin < (int64_t)(at + mine) * p.hkv)
+      for (int s = s_lo; s < s_hi; ++s) {
+        const int n = span_of(p, s, R).tiles;
+        if (begin < (int64_t)(at + n) * p.hkv) {
+          S.first_seq = s;
+          S.first_prefix = at;
+          break;
+        }
+        at += n;
+      }
+  }
+  // queries of sequences without a key: zeros
+  for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
+    const Span sp = span_of(p, s, R);
+    if (sp.tiles == 0 && sp.qlen > 0 && sp.qlen <= R && sp.qlen * p.group <= R)
+      for (int i = tid; i < sp.qlen * p.hkv * p.group * kHead; i += kThreads) {
+        const int t = i / (p.hkv * p.group * kHead), h = i / kHead % (p.hkv * p.group);
+        p.out[(int64_t)(sp.row0 + t) * p.o_st + (int64_t)h * p.o_sh + i % kHead] = __float2bfloat16_rn(0.f);
+      }
+  }
+  __syncthreads();
+  const uint32_t tbase = S.tmem;  // LK score tiles, O of group 0 and 1: N columns each
+
+  if (!busy) {
+  } else if (warp == kSoftWarps) {
+    // ---------------- TMA producer ------------------------------------------------------
+    const int ppt = kTile >> p.shift, bs = 1 << p.shift;
+    const int tpw = 32 / ppt;  // tiles whose pages the lanes hold at a time
+    if (lane == 0) {
+      tma_prefetch_desc(&kmap);
+      tma_prefetch_desc(&vmap);
+    }
+    int i = 0;
+    bool ok = true;
+    for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0 && ok; w.next()) {
+      const int n = w.count();
+      const int32_t* row = p.bt + (int64_t)w.seq * p.bt_stride;
+      auto entry = [&](int j0) {  // block of this lane's page of tiles j0 ..
+        const int j = j0 + lane / ppt;
+        if (j >= n) return -1;
+        const int page = w.s.tile(w.off + j) * ppt + lane % ppt;
+        return page << p.shift < w.s.kv_end ? __ldg(row + page) : -1;
+      };
+      int cur = entry(0), nxt = entry(tpw);
+      for (int j = 0; j < n; ++j, ++i) {
+        const int st = i % NS, j0 = j % tpw;
+        if (j > 0 && j0 == 0) {
+          cur = nxt;
+          nxt = entry(j + tpw);
+        }
+        int free = 1;
+        if (lane == 0 && i >= NS) free = mbar_wait_bounded(&S.kv_empty[st], (i / NS - 1) & 1);
+        if (!__shfl_sync(0xffffffffu, free, 0)) {
+          ok = false;
+          break;
+        }
+        const int keys = min(kTile, w.s.kv_end - w.s.tile(w.off + j) * kTile);
+        const int pages = (keys + bs - 1) >> p.shift;
+        if (lane == 0) mbar_arrive_expect_tx(&S.kv_full[st], (uint32_t)(pages * bs * kHead * 2));
+        __syncwarp();
+        const int pg = lane - j0 * ppt;
+        if (pg >= 0 && pg < pages) {
+          uint8_t* kd = smem + st * 2 * kHalf + pg * bs * kHead;
+          tma_load_4d(kd, &kmap, 0, w.kh, 0, cur, &S.kv_full[st]);
+          tma_load_4d(kd + kHalf, &vmap, 0, w.kh, 0, cur, &S.kv_full[st]);
+          const bool in = cur >= 0 && cur < p.num_blocks;  // else the block reads as zeros
+          const int64_t blk = in ? cur : 0;
+          async_word(&S.scale[st][0][pg], p.ks + blk * p.ks0 + (int64_t)w.kh * p.ks1, in);
+          async_word(&S.scale[st][1][pg], p.vs + blk * p.vs0 + (int64_t)w.kh * p.vs1, in);
+        }
+        async_arrive(&S.kv_full[st]);
+      }
+    }
+    // every copy issued has landed before the CTA may exit
+    if (lane == 0)
+      for (int j = max(0, i - NS); j < i; ++j) mbar_wait_bounded(&S.kv_full[j % NS], (j / NS) & 1);
+    __syncwarp();
+  } else if (warp == kSoftWarps + 1) {
+    // ---------------- MMA issuer --------------------------------------------------------
+    if (lane == 0) {
+      constexpr uint32_t kIdescQK = tc::idesc_f16_f32(kTile, N, false);
+      constexpr uint32_t kIdescPV = tc::idesc_f16_f32(kHead, N, false) | tc::kIdescAMnMajor;
+      const uint32_t a_kv = smem_u32(smem), a_q = smem_u32(smem + SH::kOffQ), a_p = smem_u32(smem + SH::kOffP);
+      bool failed = false;
+      int i0 = 0, seg = 0;
+      for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0; w.next(), ++seg) {
+        const int n = w.count();
+        if (!failed) failed = !mbar_wait_bounded(&S.q_full[seg & 1], (seg >> 1) & 1);
+        auto qk = [&](int j) {
+          const int i = i0 + j, st = i % NS;
+          if (!failed) failed = !mbar_wait_bounded(&S.kv_full[st], (i / NS) & 1);
+          if (!failed) {
+            tc::fence_after_sync();
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              tc::mma_f8(tbase + (i % LK) * N, tc::sdesc_sw128(a_kv + st * 2 * kHalf + ks * 32, 16, 1024),
+                         tc::sdesc_sw128(a_q + (seg & 1) * SH::kOperand + ks * 32, 16, 1024), kIdescQK, ks != 0);
+          }
+          tc::commit(&S.s_full[i % LK]);
+        };
+        auto pv = [&](int j) {
+          const int i = i0 + j, st = i % NS, X = i & 1;
+          if (!failed) failed = !mbar_wait_bounded(&S.p_full[X], (i >> 1) & 1);
+          if (!failed) {
+            tc::fence_after_sync();
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              tc::mma_f8(tbase + LK * N + X * N,
+                         tc::sdesc_sw128(a_kv + st * 2 * kHalf + kHalf + ks * 32 * 128, kHalf, 1024),
+                         tc::sdesc_sw128(a_p + X * SH::kOperand + ks * 32, 16, 1024), kIdescPV, j > 1 || ks != 0);
+          }
+          tc::commit(&S.pv_done[X]);
+          tc::commit(&S.kv_empty[st]);
+        };
+        for (int j = 0; j < min(n, LK); ++j) qk(j);
+        for (int j = 0; j < n; ++j) {
+          pv(j);  // its P was made from score tile j, which is free now
+          if (j + LK < n) qk(j + LK);
+        }
+        i0 += n;
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax groups ----------------------------------------------------
+    const int X = warp / kGroupWarps, gw = warp % kGroupWarps, gt = tid % (kGroupWarps * 32);
+    const uint32_t lane_off = (uint32_t)(gw * 32) << 16;
+    const uint32_t t_o = tbase + LK * N + X * N + lane_off;
+    uint8_t* sp = smem + SH::kOffP + X * SH::kOperand;
+    float* join = reinterpret_cast<float*>(smem + SH::kOffP);  // [R][kHead]
+    bool failed = false;
+    int i0 = 0, seg = 0;
+    for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0; w.next(), ++seg) {
+      const int n = w.count(), qb = seg & 1;
+      const Span& s = w.s;
+      const int rows = s.qlen * p.group;
+      // ---- Q: per-row power-of-two prescale (maximum in [2^7, 2^8)), two terms -----------
+      for (int e = tid; e < R * 8; e += kSoftWarps * 32) {
+        const int r = e >> 3, c = e & 7, t = r / p.group;
+        uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (r < rows) {
+          const uint4* src = reinterpret_cast<const uint4*>(
+              p.q + (int64_t)(s.row0 + t) * p.q_st + (int64_t)(w.kh * p.group + r - t * p.group) * p.q_sh + 16 * c);
+          raw[0] = src[0];
+          raw[1] = src[1];
+        }
+        float v[16], mx = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t u[4] = {raw[h].x, raw[h].y, raw[h].z, raw[h].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            v[8 * h + 2 * k] = __uint_as_float(u[k] << 16);
+            v[8 * h + 2 * k + 1] = __uint_as_float(u[k] & 0xFFFF0000u);
+            mx = fmaxf(mx, fmaxf(fabsf(v[8 * h + 2 * k]), fabsf(v[8 * h + 2 * k + 1])));
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const int E = (int)((__float_as_uint(mx) >> 23) & 0xFF);
+        int sh = (E == 0xFF || mx == 0.f) ? 0 : 134 - E;
+        sh = max(-126, min(126, sh));
+        const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] *= up;
+        uint4 hi, lo;
+        pack16<(int)kLo>(v, hi, lo);
+        uint8_t* q = smem + SH::kOffQ + qb * SH::kOperand;
+        *reinterpret_cast<uint4*>(q + swz(r, c)) = hi;
+        *reinterpret_cast<uint4*>(q + swz(R + r, c)) = lo;
+        if (c == 0) {
+          S.factor[qb][r] = p.sm_scale * kLog2e * __uint_as_float((uint32_t)(127 - sh) << 23);
+          S.pos[qb][r] = r < rows ? s.q0 + t : 0x7FFFFFFF;
+        }
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.q_full[qb]);
+      named_bar_sync(3, kSoftWarps * 32);  // factor and pos are visible
+
+      float l[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) l[r] = 0.f;
+      const int first = (i0 ^ X) & 1;  // the segment's first tile of this group
+      if (gt < R) S.ref[X][((i0 + first) >> 1) & 1][gt] = -INFINITY;
+      for (int j = first; j < n; j += 2) {
+        const int i = i0 + j, st = i % NS, k = i >> 1;  // k: count of the group's tiles
+        const int key0 = s.tile(w.off + j) * kTile, key = key0 + gt;
+        const uint32_t t_s = tbase + (i % LK) * N + lane_off;
+        if (!failed) failed = !mbar_wait_bounded(&S.s_full[i % LK], (i / LK) & 1);
+        tc::fence_after_sync();
+        // all rows see the whole tile, or the mask is asked
+        const bool open = key0 + kTile - 1 <= s.q0 && key0 + kTile <= s.kv_end &&
+                          (p.window == 0 || key0 > s.total - 1 - p.window || key0 + kTile <= p.sinks);
+        const bool seen = open || (key < s.kv_end && (p.window == 0 || key > s.q0 - p.window || key < p.sinks));
+        float ks = 0.f, lvs = 0.f, inv_vs = 0.f;
+        if (seen) {
+          ks = S.scale[st][0][gt >> p.shift];
+          const float vs = fminf(fmaxf(S.scale[st][1][gt >> p.shift], kMinScale), kMaxScale);
+          lvs = __log2f(vs);
+          inv_vs = __frcp_rn(vs);
+        }
+        float x[CH];
+        auto scores = [&](int c) {  // x of rows CH c ..
+          float lo[CH];
+          tc::ld_wait(t_s + CH * c, x);
+          tc::ld_wait(t_s + R + CH * c, lo);
+#pragma unroll
+          for (int r = 0; r < CH; ++r) {
+            x[r] = fmaf(fmaf(lo[r], 1.f / kLo, x[r]) * S.factor[qb][CH * c + r], ks, lvs);
+            if (!open) {
+              const int pos = S.pos[qb][CH * c + r];
+              if (!(seen && key <= pos && (p.window == 0 || key > pos - p.window || key < p.sinks))) x[r] = -INFINITY;
+            }
+          }
+        };
+#pragma unroll
+        for (int c = 0; c < R / CH; ++c) {
+          scores(c);
+#pragma unroll
+          for (int r = 0; r < CH; ++r) {
+            const float m = warp_max(x[r]);
+            if (lane == (r & 31)) S.part_max[X][k & 1][gw][CH * c + r] = m;
+          }
+        }
+        named_bar_sync(1 + X, kGroupWarps * 32);
+        // the reference of each row, the same in every thread
+        bool moved = false;
+        float m[CH];
+        auto reference = [&](int c, bool write) {
+#pragma unroll
+          for (int r = 0; r < CH; ++r) {
+            const int a = CH * c + r;
+            const float top = fmaxf(fmaxf(S.part_max[X][k & 1][0][a], S.part_max[X][k & 1][1][a]),
+                                    fmaxf(S.part_max[X][k & 1][2][a], S.part_max[X][k & 1][3][a]));
+            const float old = S.ref[X][k & 1][a];
+            m[r] = top > old + kLazy ? top : old;
+            if (write) {
+              moved |= m[r] != old;
+              if (gt == a) S.ref[X][(k & 1) ^ 1][a] = m[r];
+            }
+          }
+        };
+#pragma unroll
+        for (int c = 0; c < R / CH; ++c) reference(c, true);
+        // the group's previous product is done: P is free and O is stable
+        if (k > 0 && !failed) failed = !mbar_wait_bounded(&S.pv_done[X], (k - 1) & 1);
+        tc::fence_after_sync();
+        if (moved && j > first) {
+          auto rescale = [&](uint32_t addr, const float (&a)[CH]) {
+            float o[CH];
+            tc::ld_wait(addr, o);
+#pragma unroll
+            for (int r = 0; r < CH; ++r) o[r] *= a[r];
+            tc::st(addr, o);
+          };
+#pragma unroll
+          for (int c = 0; c < R / CH; ++c) {
+            float a[CH];
+            reference(c, false);
+#pragma unroll
+            for (int r = 0; r < CH; ++r) {
+              const float old = S.ref[X][k & 1][CH * c + r];
+              a[r] = m[r] == old ? 1.f : ex2(old - m[r]);
+              l[CH * c + r] *= a[r];
+            }
+            rescale(t_o + CH * c, a);
+            rescale(t_o + R + CH * c, a);
+          }
+          tc::wait_st();
+        }
+#pragma unroll
+        for (int c = 0; c < R / CH; ++c) {
+          if constexpr (R > CH) {
+            scores(c);
+            reference(c, false);
+          }
+#pragma unroll
+          for (int r = 0; r < CH; ++r) {
+            const int a = CH * c + r;
+            const float pr = ex2(x[r] - (m[r] == -INFINITY ? 0.f : m[r] - kOff));
+            l[a] = fmaf(pr, inv_vs, l[a]);
+            float hi, lo;
+            split4(pr, hi, lo);
+            const uint32_t b = e4m3x2(hi, lo * kLo);
+            sp[swz(a, gt >> 4) + (gt & 15)] = (uint8_t)b;
+            sp[swz(R + a, gt >> 4) + (gt & 15)] = (uint8_t)(b >> 8);
+          }
+        }
+        if (!seen) {
+          uint4* v = reinterpret_cast<uint4*>(smem + st * 2 * kHalf + kHalf + gt * kHead);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[c] = make_uint4(0, 0, 0, 0);
+        }
+        tc::fence_proxy_async_smem();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.p_full[X]);
+      }
+
+      // ---- the segment's end: join the groups, store or leave a partial ------------------
+      const int own = (n - first + 1) / 2;  // tiles of this group
+      const int klast = (i0 + first + 2 * (own - 1)) >> 1;
+      if (own > 0 && !failed) failed = !mbar_wait_bounded(&S.pv_done[X], klast & 1);
+      tc::fence_after_sync();
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float v = l[r];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == (r & 31)) S.fin_l[X][gw][r] = v;
+      }
+      if (gt < R) S.fin_m[X][gt] = own > 0 ? S.ref[X][(klast & 1) ^ 1][gt] : -INFINITY;
+      named_bar_sync(3, kSoftWarps * 32);
+      auto weight = [&](int g, int r) {  // of group g in row r's sum
+        const float a = S.fin_m[g][r], b = S.fin_m[g ^ 1][r];
+        return a == -INFINITY ? 0.f : ex2(a - fmaxf(a, b));
+      };
+      auto output = [&](int c, float (&o)[CH]) {  // this group's O^T of rows CH c .., dimension gt
+        float lo[CH];
+        tc::ld_wait(t_o + CH * c, o);
+        tc::ld_wait(t_o + R + CH * c, lo);
+#pragma unroll
+        for (int r = 0; r < CH; ++r) o[r] = fmaf(lo[r], 1.f / kLo, o[r]) * weight(X, CH * c + r);
+      };
+      if (X == 1 && own > 0) {
+#pragma unroll
+        for (int c = 0; c < R / CH; ++c) {
+          float o[CH];
+          output(c, o);
+#pragma unroll
+          for (int r = 0; r < CH; ++r) join[(CH * c + r) * kHead + gt] = o[r];
+        }
+      }
+      const bool other = n - ((i0 ^ 1) & 1) > 0;  // group 1 had a tile
+      named_bar_sync(3, kSoftWarps * 32);
+      if (X == 0 && (own > 0 || other)) {
+#pragma unroll
+        for (int c = 0; c < R / CH; ++c) {
+          float o[CH];
+          if (own > 0) output(c, o);
+#pragma unroll
+          for (int r = 0; r < CH; ++r) {
+            const int a = (CH * c + r) * kHead + gt;
+            if (own > 0) join[a] = other ? join[a] + o[r] : o[r];
+          }
+        }
+      }
+      named_bar_sync(3, kSoftWarps * 32);
+      auto store = [&](int a, int c, float4 o, float sum) {  // row a, dimensions 4 c ..
+        const float f = sum > 0.f ? __fdividef(1.f, sum) : 0.f;
+        const int t = a / p.group;
+        const __nv_bfloat162 u = __floats2bfloat162_rn(o.x * f, o.y * f), v = __floats2bfloat162_rn(o.z * f, o.w * f);
+        *reinterpret_cast<uint2*>(p.out + (int64_t)(s.row0 + t) * p.o_st +
+                                  (int64_t)(w.kh * p.group + a - t * p.group) * p.o_sh + 4 * c) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
+      };
+      const bool whole = n == s.tiles;
+      constexpr int kPart = kMaxRows * (kHead + 2);
+      float* part = p.partials + (int64_t)(2 * blockIdx.x + (w.item >= begin ? 1 : 0)) * kPart;
+      for (int e = tid; e < rows * (kHead / 4); e += kSoftWarps * 32) {
+        const int a = e / (kHead / 4), c = e % (kHead / 4);
+        const float4 o = *reinterpret_cast<const float4*>(join + a * kHead + 4 * c);
+        float sum = 0.f;
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          sum += weight(g, a) * (S.fin_l[g][0][a] + S.fin_l[g][1][a] + S.fin_l[g][2][a] + S.fin_l[g][3][a]);
+        if (whole) {
+          store(a, c, o, sum);
+        } else {
+          *reinterpret_cast<float4*>(part + a * kHead + 4 * c) = o;
+          if (c == 0)
+            *reinterpret_cast<float2*>(part + kMaxRows * kHead + 2 * a) =
+                make_float2(fmaxf(S.fin_m[0][a], S.fin_m[1][a]), sum);
+        }
+      }
+      if (!whole) {
+        __threadfence();
+        named_bar_sync(3, kSoftWarps * 32);
+        const int c_lo = share_owner(w.item, total, ctas), c_hi = share_owner(w.item + s.tiles - 1, total, ctas);
+        if (tid == 0) {
+          int* counter = p.counters + (int64_t)w.seq * p.hkv + w.kh;
+          S.last = atomicAdd(counter, 1) == c_hi - c_lo;
+          if (S.last) *counter = 0;
+        }
+        named_bar_sync(3, kSoftWarps * 32);
+        if (S.last) {
+          __threadfence();
+          // the shares of the item in order, kJoin loads of each kind in flight
+          constexpr int kJoin = 8;
+          const int slot0 = 2 * c_lo + (w.item >= share_begin(c_lo, total, ctas) ? 1 : 0);  // later ones begin inside it
+          for (int e = tid; e < rows * (kHead / 4); e += kSoftWarps * 32) {
+            const int a = e / (kHead / 4), c = e % (kHead / 4);
+            float top = -INFINITY, sum = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int c0 = c_lo; c0 <= c_hi; c0 += kJoin) {
+              float2 ml[kJoin];
+              float4 v[kJoin];
+              float nt = top;
+#pragma unroll
+              for (int u = 0; u < kJoin; ++u) {
+                ml[u] = make_float2(-INFINITY, 0.f);
+                if (c0 + u <= c_hi) {
+                  const float* q = p.partials + (int64_t)(c0 + u == c_lo ? slot0 : 2 * (c0 + u)) * kPart;
+                  ml[u] = __ldcg(reinterpret_cast<const float2*>(q + kMaxRows * kHead + 2 * a));
+                  v[u] = __ldcg(reinterpret_cast<const float4*>(q + a * kHead + 4 * c));
+                }
+              }
+#pragma unroll
+              for (int u = 0; u < kJoin; ++u) nt = fmaxf(nt, ml[u].x);
+              if (nt == -INFINITY) continue;
+              const float f = ex2(top - nt);
+              sum *= f;
+              o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+              for (int u = 0; u < kJoin; ++u)
+                if (ml[u].x != -INFINITY) {
+                  const float g = ex2(ml[u].x - nt);
+                  sum = fmaf(g, ml[u].y, sum);
+                  o.x = fmaf(g, v[u].x, o.x); o.y = fmaf(g, v[u].y, o.y);
+                  o.z = fmaf(g, v[u].z, o.z); o.w = fmaf(g, v[u].w, o.w);
+                }
+              top = nt;
+            }
+            store(a, c, o, sum);
+          }
+        }
+      }
+      named_bar_sync(3, kSoftWarps * 32);  // P and the exchange buffers are free
+      i0 += n;
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == kSoftWarps + 1) tc::tmem_dealloc(tbase, SH::kTmem);
+}
+
+template <int R>
+cudaError_t launch(const CUtensorMap& km, const CUtensorMap& vm, const BlockAttnParams& p, int ctas, cudaStream_t st) {
+  const int smem = Shape<R>::kBytes + 1024;
+  const cudaError_t e =
+      cudaFuncSetAttribute(block_decode_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(ctas, 1, 1);
+  lc.blockDim = dim3(kThreads, 1, 1);
+  lc.dynamicSmemBytes = smem;
+  lc.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = attr;
+  lc.numAttrs = pdl_enabled() ? 1 : 0;
+  return cudaLaunchKernelEx(&lc, block_decode_kernel<R>, km, vm, p);
+}
+
+}  // namespace
+
+cudaError_t block_decode_launch(const CUtensorMap& km, const CUtensorMap& vm, const BlockAttnParams& p, int rows,
+                                cudaStream_t st) {
+  const int ctas = num_sms_current_device() < kMaxCtas ? num_sms_current_device() : kMaxCtas;
+  if (rows <= 8) return launch<8>(km, vm, p, ctas, st);
+  if (rows <= 16) return launch<16>(km, vm, p, ctas, st);
+  if (rows <= 32) return launch<32>(km, vm, p, ctas, st);
+  return launch<64>(km, vm, p, ctas, st);
+}
+
+}  // namespace b200kv

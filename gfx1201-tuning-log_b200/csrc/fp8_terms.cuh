@@ -1,0 +1,54 @@
+// Two-term e4m3 operands of the attention kernels on 8-bit tcgen05 MMAs: a value
+// of 8 significant bits as hi + lo, both e4m3, and the swizzled tiles they live in.
+#pragma once
+
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+namespace b200kv {
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// (a, b) -> two e4m3 bytes, a in the low byte.
+__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+// Split x into hi + lo with hi = x rounded to 4 significant bits (half away
+// from zero on the magnitude; exact in e4m3 when |x| >= 2^-6) and lo = x - hi
+// (exact in fp32, |lo| <= 2^-4 |x|), so hi + e4m3(lo) carries x to 2^-8.
+__device__ __forceinline__ void split4(float x, float& hi, float& lo) {
+  hi = __uint_as_float((__float_as_uint(x) + 0x00080000u) & 0xFFF00000u);
+  lo = x - hi;
+}
+
+// 16 floats -> 16 e4m3 bytes of hi and of lo * LO_SCALE (element 0 in the
+// lowest byte).
+template <int LO_SCALE>
+__device__ __forceinline__ void pack16(const float* v, uint4& hi, uint4& lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    float a0, a1, a2, a3, b0, b1, b2, b3;
+    split4(v[4 * w + 0], a0, b0);
+    split4(v[4 * w + 1], a1, b1);
+    split4(v[4 * w + 2], a2, b2);
+    split4(v[4 * w + 3], a3, b3);
+    constexpr float ls = (float)LO_SCALE;
+    h[w] = e4m3x2(a0, a1) | (e4m3x2(a2, a3) << 16);
+    l[w] = e4m3x2(b0 * ls, b1 * ls) | (e4m3x2(b2 * ls, b3 * ls) << 16);
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+// byte offset of 16-byte chunk c of row r in a 128-byte-swizzled [rows][128 B] tile
+__device__ __forceinline__ uint32_t swz(int r, int c) {
+  return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
+}
+
+}  // namespace b200kv
