@@ -27,12 +27,13 @@ struct BlockAttnParams {
   int64_t sk0, sk1, sk2, sv0, sv1, sv2, ks0, ks1, vs0, vs1;
   float sm_scale;
   int num_seqs, hkv, group, shift, num_blocks, max_blocks, window, sinks;
+  int heads, slots;  // of the few-query kernel: kv heads a CTA walks, CTAs that share a range
   float* partials;  // [2 kMaxCtas][kMaxRows x (128 + m + l)]
   int* counters;    // [num_seqs][hkv], zero between calls
 };
 
 // sequences with at most kMaxRows rows per kv head; `rows` bounds them in this batch
-cudaError_t block_decode_launch(const CUtensorMap& km, const CUtensorMap& vm, const BlockAttnParams& p, int rows,
+cudaError_t block_decode_launch(const CUtensorMap& km, const CUtensorMap& vm, BlockAttnParams p, int rows,
                                 cudaStream_t st);
 
 }  // namespace b200kv

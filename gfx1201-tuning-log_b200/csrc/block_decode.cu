@@ -18,16 +18,24 @@
 // One CTA per SM walks a contiguous range of the batch's tiles, ordered by
 // (sequence, kv head, tile) and cut into equal shares on the device from the
 // lengths, so a ragged batch keeps every SM equally busy and the K/V ring never
-// drains between items.  Shares that cut an item leave (o, m, l) in the workspace;
-// the last CTA of the item to finish (a counter, back at zero afterwards) joins
-// them in order, so the sum does not depend on who is last.
+// drains between items.  A share is walked by `slots` CTAs at once, one for each kv
+// head (or few): the heads of a block lie side by side in memory, and reading them
+// at the same time is worth 4.4 -> 6.7 TB/s (blocks of 64 tokens, loads alone).
+// Shares that cut an item leave (o, m, l) in the workspace; the last CTA of the
+// item to finish (a counter, back at zero afterwards) joins them in order, so the
+// sum does not depend on who is last.
 //
-// Roles: 8 softmax warps in two groups that take alternate tiles (own S, O, P and
-// running state each, joined at the item's end), a TMA warp, an MMA warp.  A
-// softmax thread is one key: it reads its row of S^T, the group finds each row's
-// maximum (a warp maximum and an exchange through shared memory), and P goes to
-// shared memory as the K-major B operand.  Keys no query sees have their V rows
-// zeroed, so stale or non-finite codes never reach an output.
+// Roles: 8 softmax warps in two groups that take alternate tiles (own O, P and
+// running state each, joined at the item's end), a TMA warp for K and one for V, a
+// warp that issues the first product and one that issues the second (a thread
+// issues an MMA in about 100 cycles: one issuer for all eight of a tile, or one TMA
+// warp for its sixteen 2 KB pages, bounds the kernel).
+// A softmax thread is one key: it reads its row of S^T and one vote of the group
+// asks whether any score passes its row's reference by 2^4; only then are the
+// maxima found and O rescaled, on a segment's first tile and rarely after it.  P
+// goes to shared memory as the MN-major B operand, a thread's row in 16-byte
+// stores.  Keys no query sees have their V rows zeroed, so stale or non-finite
+// codes never reach an output.
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -49,7 +57,9 @@ constexpr int kTile = 128;                  // keys per tile
 constexpr int kHalf = kTile * kHead;        // K (or V) bytes of a tile
 constexpr int kGroupWarps = 4;
 constexpr int kSoftWarps = 2 * kGroupWarps;
-constexpr int kThreads = (kSoftWarps + 2) * 32;
+constexpr int kQkWarp = kSoftWarps, kPvWarp = kSoftWarps + 1, kTmaWarp = kSoftWarps + 2;  // K's, then V's
+constexpr int kWarps = kSoftWarps + 4;
+constexpr int kThreads = kWarps * 32;
 constexpr int kMaxPages = 8;                // pages per tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 4.f;                // the reference moves when a maximum exceeds it by 2^4
@@ -57,6 +67,8 @@ constexpr float kOff = 4.f;                 // P is formed times 2^4 (at most 2^
 constexpr float kLo = 16.f;                 // the second terms carry 16 times the remainder
 constexpr float kMinScale = 8.2718061e-25f; // 2^-80
 constexpr float kMaxScale = 1.2089258e24f;  // 2^80
+constexpr float kMasked = -3e38f;           // the score of a key that a query does not see
+constexpr float kNone = -1e30f;             // the reference of a row that has seen no key
 
 template <int R>
 struct Shape {
@@ -64,29 +76,54 @@ struct Shape {
   static constexpr int kStages = R >= 64 ? 4 : R == 32 ? 5 : 6;
   static constexpr int kOperand = kN * 128; // bytes of Q or P
   static constexpr int kOffQ = kStages * 2 * kHalf;  // [segment parity]
-  static constexpr int kOffP = kOffQ + 2 * kOperand; // [group]; the groups' join at a segment's end
+  static constexpr int kOffP = kOffQ + 2 * kOperand; // [group][key][N]; the groups' join at a segment's end
   static constexpr int kBytes = kOffP + 2 * kOperand;
   static constexpr int kChunk = R < 16 ? R : 16;     // rows handled together
   static constexpr int kLook = R >= 64 ? 2 : 4;      // score tiles in tensor memory
   static constexpr uint32_t kTmem = R == 8 ? 128 : R == 16 ? 256 : 512;  // kLook S + 2 O tiles of N columns
+  // P rows of N bytes, swizzled over their width (none, 32, 64, 128 bytes)
+  static constexpr uint32_t kLayoutP = R == 8 ? 0 : R == 16 ? 6 : R == 32 ? 4 : 2;
+  __device__ static __forceinline__ uint32_t p_at(int key, int chunk) {
+    return key * kN + ((chunk ^ ((key * kN >> 7) & (kN / 16 - 1))) << 4);
+  }
+  __device__ static __forceinline__ uint64_t p_desc(uint32_t addr) {  // 8-key groups 8 N bytes apart
+    return R == 8 ? tc::sdesc(addr, 8 * kN, 16, kLayoutP) : tc::sdesc(addr, 16, 8 * kN, kLayoutP);
+  }
   static_assert((kLook + 2) * kN <= (int)kTmem && kStages > kLook, "tensor memory; a stage free to load into");
 };
 
 template <int R>
 struct Shared {
   uint64_t kv_full[Shape<R>::kStages], kv_empty[Shape<R>::kStages];
-  uint64_t q_full[2], s_full[Shape<R>::kLook], p_full[2], pv_done[2];
+  uint64_t q_full[2], s_full[Shape<R>::kLook], s_free[Shape<R>::kLook], p_full[2], pv_done[2];
   uint32_t tmem;
   float scale[Shape<R>::kStages][2][kMaxPages];      // ks, vs of a tile's pages
   alignas(16) float factor[2][R];                    // [segment parity] score factor of a row
   alignas(16) int pos[2][R];                         // and its position
-  alignas(16) float part_max[2][2][kGroupWarps][R];  // [group][tile parity][warp]
-  alignas(16) float ref[2][2][R];                    // [group][tile parity] the reference m
+  alignas(16) float part_max[2][kGroupWarps][R];     // [group][warp]
+  alignas(16) float ref[2][R];                       // [group] P = 2^(x - ref)
+  alignas(16) float alpha[2][R];                     // and what its last move scales O and l by
   alignas(16) float fin_m[2][R], fin_l[2][kGroupWarps][R];
   int first_seq, first_prefix, last;
-  int warp_sum[kSoftWarps + 2];
+  int warp_sum[kWarps];
 };
 
+// CH per-row values from shared memory (16-byte aligned)
+template <int CH>
+__device__ __forceinline__ void row_values(float (&v)[CH], const float* src) {
+#pragma unroll
+  for (int i = 0; i < CH; i += 4) *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(src + i);
+}
+// Named barrier over `count` threads that ORs a predicate.
+__device__ __forceinline__ bool named_bar_or(int id, int count, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"(pred ? 1u : 0u), "r"(id), "r"(count)
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ float warp_max(float x) {
   float r;
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
@@ -127,29 +164,31 @@ __device__ __forceinline__ Span span_of(const BlockAttnParams& p, int seq, int m
   return s;
 }
 
-// A CTA's share, segment by segment (a segment: consecutive tiles of one item).
+// A CTA's share, segment by segment (a segment: consecutive tiles of one item, an
+// item: a sequence and kv head).
 struct Walk {
   const BlockAttnParams& p;
   int max_rows;
   Span s;
-  int seq, kh, off, left;
-  int64_t item;  // index of the item's first tile among the batch's
+  int seq, sub, off, left;  // sub: which of the CTA's p.heads kv heads
+  int64_t item;  // index of the item's first tile in the slot's order
   __device__ Walk(const BlockAttnParams& p_, int max_rows_, int seq_, int prefix, int64_t begin, int count)
       : p(p_), max_rows(max_rows_), seq(seq_), left(count) {
     s = span_of(p, seq, max_rows);
-    const int rel = (int)(begin - (int64_t)prefix * p.hkv);
-    kh = rel / s.tiles;
-    off = rel - kh * s.tiles;
+    const int rel = (int)(begin - (int64_t)prefix * p.heads);
+    sub = rel / s.tiles;
+    off = rel - sub * s.tiles;
     item = begin - off;
   }
   __device__ __forceinline__ int count() const { return min(s.tiles - off, left); }
+  __device__ __forceinline__ int kh() const { return blockIdx.x % p.slots * p.heads + sub; }
   __device__ __forceinline__ void next() {
     left -= count();
     if (left <= 0) return;
     item += s.tiles;
     off = 0;
-    if (++kh == p.hkv) {
-      kh = 0;
+    if (++sub == p.heads) {
+      sub = 0;
       do {
         s = span_of(p, ++seq, max_rows);
       } while (s.tiles == 0 && seq + 1 < p.num_seqs);
@@ -157,9 +196,11 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ int64_t share_begin(int64_t cta, int64_t total, int64_t ctas) { return cta * total / ctas; }
-__device__ __forceinline__ int share_owner(int64_t tile, int64_t total, int64_t ctas) {
-  return (int)(((tile + 1) * ctas - 1) / total);
+__device__ __forceinline__ int64_t share_begin(int64_t share, int64_t total, int64_t shares) {
+  return share * total / shares;
+}
+__device__ __forceinline__ int share_owner(int64_t tile, int64_t total, int64_t shares) {
+  return (int)(((tile + 1) * shares - 1) / total);
 }
 
 template <int R>
@@ -176,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     griddep_launch_dependents();
     for (int s = 0; s < NS; ++s) {
-      mbar_init(&S.kv_full[s], 1 + 32);  // the bytes of the tile, and each producer lane's scales
+      mbar_init(&S.kv_full[s], 2 * (1 + 32));  // K's and V's bytes, and each producer lane's scales
       mbar_init(&S.kv_empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -184,10 +225,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&S.p_full[b], kGroupWarps);
       mbar_init(&S.pv_done[b], 1);
     }
-    for (int b = 0; b < LK; ++b) mbar_init(&S.s_full[b], 1);
+    for (int b = 0; b < LK; ++b) {
+      mbar_init(&S.s_full[b], 1);
+      mbar_init(&S.s_free[b], kGroupWarps);
+    }
     fence_mbar_init();
   }
-  if (warp == kSoftWarps + 1) tc::tmem_alloc(&S.tmem, SH::kTmem);
+  if (warp == kQkWarp) tc::tmem_alloc(&S.tmem, SH::kTmem);
   griddep_wait();  // lengths, tables and q may be the previous kernel's
 
   // ---- this CTA's share: an inclusive scan of the sequences' tile counts -------------
@@ -207,21 +251,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after_sync();
   int before = 0, tiles = 0;
 #pragma unroll
-  for (int w = 0; w < kSoftWarps + 2; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += S.warp_sum[w];
     tiles += S.warp_sum[w];
   }
-  const int64_t total = (int64_t)tiles * p.hkv;
-  const int64_t ctas = min((int64_t)gridDim.x, total);
-  const bool busy = blockIdx.x < ctas;
-  const int64_t begin = busy ? share_begin(blockIdx.x, total, ctas) : 0;
-  const int count = busy ? (int)(share_begin(blockIdx.x + 1, total, ctas) - begin) : 0;
+  const int64_t total = (int64_t)tiles * p.heads;
+  const int slot = blockIdx.x % p.slots, share = blockIdx.x / p.slots;
+  const int64_t shares = min((int64_t)(gridDim.x / p.slots), total);
+  const bool busy = share < shares;
+  const int64_t begin = busy ? share_begin(share, total, shares) : 0;
+  const int count = busy ? (int)(share_begin(share + 1, total, shares) - begin) : 0;
   if (busy) {
     int at = before + incl - mine;  // tiles of the sequences before this thread's
-    if (begin >= (int64_t)at * p.hkv && begin < (int64_t)(at + mine) * p.hkv)
+    if (begin >= (int64_t)at * p.heads && begin < (int64_t)(at + mine) * p.heads)
       for (int s = s_lo; s < s_hi; ++s) {
         const int n = span_of(p, s, R).tiles;
-        if (begin < (int64_t)(at + n) * p.hkv) {
+        if (begin < (int64_t)(at + n) * p.heads) {
           S.first_seq = s;
           S.first_prefix = at;
           break;
@@ -242,18 +287,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tbase = S.tmem;  // LK score tiles, O of group 0 and 1: N columns each
 
   if (!busy) {
-  } else if (warp == kSoftWarps) {
-    // ---------------- TMA producer ------------------------------------------------------
+  } else if (warp >= kTmaWarp) {
+    // ---------------- TMA producers: K pages, V pages -----------------------------------
+    const bool is_v = warp > kTmaWarp;
+    const CUtensorMap* map = is_v ? &vmap : &kmap;
+    const float* scales = is_v ? p.vs : p.ks;
+    const int64_t sc0 = is_v ? p.vs0 : p.ks0, sc1 = is_v ? p.vs1 : p.ks1;
     const int ppt = kTile >> p.shift, bs = 1 << p.shift;
     const int tpw = 32 / ppt;  // tiles whose pages the lanes hold at a time
-    if (lane == 0) {
-      tma_prefetch_desc(&kmap);
-      tma_prefetch_desc(&vmap);
-    }
+    if (lane == 0) tma_prefetch_desc(map);
     int i = 0;
     bool ok = true;
     for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0 && ok; w.next()) {
-      const int n = w.count();
+      const int n = w.count(), kh = w.kh();
       const int32_t* row = p.bt + (int64_t)w.seq * p.bt_stride;
       auto entry = [&](int j0) {  // block of this lane's page of tiles j0 ..
         const int j = j0 + lane / ppt;
@@ -276,17 +322,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int keys = min(kTile, w.s.kv_end - w.s.tile(w.off + j) * kTile);
         const int pages = (keys + bs - 1) >> p.shift;
-        if (lane == 0) mbar_arrive_expect_tx(&S.kv_full[st], (uint32_t)(pages * bs * kHead * 2));
+        if (lane == 0) mbar_arrive_expect_tx(&S.kv_full[st], (uint32_t)(pages * bs * kHead));
         __syncwarp();
         const int pg = lane - j0 * ppt;
         if (pg >= 0 && pg < pages) {
-          uint8_t* kd = smem + st * 2 * kHalf + pg * bs * kHead;
-          tma_load_4d(kd, &kmap, 0, w.kh, 0, cur, &S.kv_full[st]);
-          tma_load_4d(kd + kHalf, &vmap, 0, w.kh, 0, cur, &S.kv_full[st]);
+          tma_load_4d(smem + st * 2 * kHalf + is_v * kHalf + pg * bs * kHead, map, 0, kh, 0, cur, &S.kv_full[st]);
           const bool in = cur >= 0 && cur < p.num_blocks;  // else the block reads as zeros
-          const int64_t blk = in ? cur : 0;
-          async_word(&S.scale[st][0][pg], p.ks + blk * p.ks0 + (int64_t)w.kh * p.ks1, in);
-          async_word(&S.scale[st][1][pg], p.vs + blk * p.vs0 + (int64_t)w.kh * p.vs1, in);
+          async_word(&S.scale[st][is_v][pg], scales + (in ? cur : 0) * sc0 + kh * sc1, in);
         }
         async_arrive(&S.kv_full[st]);
       }
@@ -295,31 +337,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0)
       for (int j = max(0, i - NS); j < i; ++j) mbar_wait_bounded(&S.kv_full[j % NS], (j / NS) & 1);
     __syncwarp();
-  } else if (warp == kSoftWarps + 1) {
-    // ---------------- MMA issuer --------------------------------------------------------
+  } else if (warp == kQkWarp) {
+    // ---------------- S^T = K Q^T -------------------------------------------------------
     if (lane == 0) {
-      constexpr uint32_t kIdescQK = tc::idesc_f16_f32(kTile, N, false);
-      constexpr uint32_t kIdescPV = tc::idesc_f16_f32(kHead, N, false) | tc::kIdescAMnMajor;
-      const uint32_t a_kv = smem_u32(smem), a_q = smem_u32(smem + SH::kOffQ), a_p = smem_u32(smem + SH::kOffP);
+      constexpr uint32_t kIdesc = tc::idesc_f16_f32(kTile, N, false);
+      const uint32_t a_kv = smem_u32(smem), a_q = smem_u32(smem + SH::kOffQ);
       bool failed = false;
-      int i0 = 0, seg = 0;
+      int i = 0, seg = 0;
       for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0; w.next(), ++seg) {
-        const int n = w.count();
         if (!failed) failed = !mbar_wait_bounded(&S.q_full[seg & 1], (seg >> 1) & 1);
-        auto qk = [&](int j) {
-          const int i = i0 + j, st = i % NS;
+        for (int j = w.count(); j > 0; --j, ++i) {
+          const int st = i % NS, b = i % LK;
           if (!failed) failed = !mbar_wait_bounded(&S.kv_full[st], (i / NS) & 1);
+          if (i >= LK && !failed) failed = !mbar_wait_bounded(&S.s_free[b], (i / LK - 1) & 1);
           if (!failed) {
             tc::fence_after_sync();
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-              tc::mma_f8(tbase + (i % LK) * N, tc::sdesc_sw128(a_kv + st * 2 * kHalf + ks * 32, 16, 1024),
-                         tc::sdesc_sw128(a_q + (seg & 1) * SH::kOperand + ks * 32, 16, 1024), kIdescQK, ks != 0);
+              tc::mma_f8(tbase + b * N, tc::sdesc_sw128(a_kv + st * 2 * kHalf + ks * 32, 16, 1024),
+                         tc::sdesc_sw128(a_q + (seg & 1) * SH::kOperand + ks * 32, 16, 1024), kIdesc, ks != 0);
           }
-          tc::commit(&S.s_full[i % LK]);
-        };
-        auto pv = [&](int j) {
-          const int i = i0 + j, st = i % NS, X = i & 1;
+          tc::commit(&S.s_full[b]);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kPvWarp) {
+    // ---------------- O^T += V^T P^T ----------------------------------------------------
+    if (lane == 0) {
+      constexpr uint32_t kIdesc = tc::idesc_f16_f32(kHead, N, true) | tc::kIdescAMnMajor;
+      const uint32_t a_kv = smem_u32(smem), a_p = smem_u32(smem + SH::kOffP);
+      bool failed = false;
+      int i = 0;
+      for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0; w.next()) {
+        const int n = w.count();
+        for (int j = 0; j < n; ++j, ++i) {
+          const int st = i % NS, X = i & 1;
           if (!failed) failed = !mbar_wait_bounded(&S.p_full[X], (i >> 1) & 1);
           if (!failed) {
             tc::fence_after_sync();
@@ -327,17 +380,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int ks = 0; ks < 4; ++ks)
               tc::mma_f8(tbase + LK * N + X * N,
                          tc::sdesc_sw128(a_kv + st * 2 * kHalf + kHalf + ks * 32 * 128, kHalf, 1024),
-                         tc::sdesc_sw128(a_p + X * SH::kOperand + ks * 32, 16, 1024), kIdescPV, j > 1 || ks != 0);
+                         SH::p_desc(a_p + X * SH::kOperand + ks * 32 * N), kIdesc, j > 1 || ks != 0);
           }
           tc::commit(&S.pv_done[X]);
           tc::commit(&S.kv_empty[st]);
-        };
-        for (int j = 0; j < min(n, LK); ++j) qk(j);
-        for (int j = 0; j < n; ++j) {
-          pv(j);  // its P was made from score tile j, which is free now
-          if (j + LK < n) qk(j + LK);
         }
-        i0 += n;
       }
     }
     __syncwarp();
@@ -351,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool failed = false;
     int i0 = 0, seg = 0;
     for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0; w.next(), ++seg) {
-      const int n = w.count(), qb = seg & 1;
+      const int n = w.count(), qb = seg & 1, kh = w.kh();
       const Span& s = w.s;
       const int rows = s.qlen * p.group;
       // ---- Q: per-row power-of-two prescale (maximum in [2^7, 2^8)), two terms -----------
@@ -360,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if (r < rows) {
           const uint4* src = reinterpret_cast<const uint4*>(
-              p.q + (int64_t)(s.row0 + t) * p.q_st + (int64_t)(w.kh * p.group + r - t * p.group) * p.q_sh + 16 * c);
+              p.q + (int64_t)(s.row0 + t) * p.q_st + (int64_t)(kh * p.group + r - t * p.group) * p.q_sh + 16 * c);
           raw[0] = src[0];
           raw[1] = src[1];
         }
@@ -396,15 +443,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&S.q_full[qb]);
-      named_bar_sync(3, kSoftWarps * 32);  // factor and pos are visible
+      if (gt < R) S.ref[X][gt] = kNone;
+      named_bar_sync(3, kSoftWarps * 32);  // factor, pos and ref are visible
 
       float l[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) l[r] = 0.f;
       const int first = (i0 ^ X) & 1;  // the segment's first tile of this group
-      if (gt < R) S.ref[X][((i0 + first) >> 1) & 1][gt] = -INFINITY;
       for (int j = first; j < n; j += 2) {
-        const int i = i0 + j, st = i % NS, k = i >> 1;  // k: count of the group's tiles
+        const int i = i0 + j, st = i % NS, k = i >> 1;  // k: the group's tiles so far
         const int key0 = s.tile(w.off + j) * kTile, key = key0 + gt;
         const uint32_t t_s = tbase + (i % LK) * N + lane_off;
         if (!failed) failed = !mbar_wait_bounded(&S.s_full[i % LK], (i / LK) & 1);
@@ -420,93 +467,108 @@ __global__ void __launch_bounds__(kThreads, 1)
           lvs = __log2f(vs);
           inv_vs = __frcp_rn(vs);
         }
-        float x[CH];
-        auto scores = [&](int c) {  // x of rows CH c ..
-          float lo[CH];
-          tc::ld_wait(t_s + CH * c, x);
-          tc::ld_wait(t_s + R + CH * c, lo);
+        constexpr bool kKeep = R <= 32;  // the scores stay in registers, else they are read again
+        float x[kKeep ? R : CH];
+        auto scores = [&](int c, float* y) {  // y: scores of rows CH c ..
+          float hi[CH], lo[CH];
+          tc::ld_wait(t_s + CH * c, t_s + R + CH * c, hi, lo);
+          float f[CH];
+          row_values(f, S.factor[qb] + CH * c);
 #pragma unroll
           for (int r = 0; r < CH; ++r) {
-            x[r] = fmaf(fmaf(lo[r], 1.f / kLo, x[r]) * S.factor[qb][CH * c + r], ks, lvs);
+            y[r] = fmaf(fmaf(lo[r], 1.f / kLo, hi[r]) * f[r], ks, lvs);
             if (!open) {
               const int pos = S.pos[qb][CH * c + r];
-              if (!(seen && key <= pos && (p.window == 0 || key > pos - p.window || key < p.sinks))) x[r] = -INFINITY;
+              if (!(seen && key <= pos && (p.window == 0 || key > pos - p.window || key < p.sinks))) y[r] = kMasked;
             }
           }
         };
+        float over = kMasked;
 #pragma unroll
         for (int c = 0; c < R / CH; ++c) {
-          scores(c);
+          float* y = kKeep ? x + CH * c : x;
+          scores(c, y);
+          float m[CH];
+          row_values(m, S.ref[X] + CH * c);
 #pragma unroll
-          for (int r = 0; r < CH; ++r) {
-            const float m = warp_max(x[r]);
-            if (lane == (r & 31)) S.part_max[X][k & 1][gw][CH * c + r] = m;
-          }
+          for (int r = 0; r < CH; ++r) over = fmaxf(over, y[r] - m[r]);
         }
-        named_bar_sync(1 + X, kGroupWarps * 32);
-        // the reference of each row, the same in every thread
-        bool moved = false;
-        float m[CH];
-        auto reference = [&](int c, bool write) {
-#pragma unroll
-          for (int r = 0; r < CH; ++r) {
-            const int a = CH * c + r;
-            const float top = fmaxf(fmaxf(S.part_max[X][k & 1][0][a], S.part_max[X][k & 1][1][a]),
-                                    fmaxf(S.part_max[X][k & 1][2][a], S.part_max[X][k & 1][3][a]));
-            const float old = S.ref[X][k & 1][a];
-            m[r] = top > old + kLazy ? top : old;
-            if (write) {
-              moved |= m[r] != old;
-              if (gt == a) S.ref[X][(k & 1) ^ 1][a] = m[r];
-            }
-          }
+        auto release = [&] {
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&S.s_free[i % LK]);
         };
-#pragma unroll
-        for (int c = 0; c < R / CH; ++c) reference(c, true);
+        if constexpr (kKeep) release();
+        const bool move = named_bar_or(1 + X, kGroupWarps * 32, over > kOff + kLazy);
         // the group's previous product is done: P is free and O is stable
         if (k > 0 && !failed) failed = !mbar_wait_bounded(&S.pv_done[X], (k - 1) & 1);
         tc::fence_after_sync();
-        if (moved && j > first) {
-          auto rescale = [&](uint32_t addr, const float (&a)[CH]) {
-            float o[CH];
-            tc::ld_wait(addr, o);
-#pragma unroll
-            for (int r = 0; r < CH; ++r) o[r] *= a[r];
-            tc::st(addr, o);
-          };
+        if (move) {
 #pragma unroll
           for (int c = 0; c < R / CH; ++c) {
-            float a[CH];
-            reference(c, false);
+            float* y = kKeep ? x + CH * c : x;
+            if constexpr (!kKeep) scores(c, y);
 #pragma unroll
             for (int r = 0; r < CH; ++r) {
-              const float old = S.ref[X][k & 1][CH * c + r];
-              a[r] = m[r] == old ? 1.f : ex2(old - m[r]);
-              l[CH * c + r] *= a[r];
+              const float m = warp_max(y[r]);
+              if (lane == (r & 31)) S.part_max[X][gw][CH * c + r] = m;
             }
-            rescale(t_o + CH * c, a);
-            rescale(t_o + R + CH * c, a);
           }
-          tc::wait_st();
+          named_bar_sync(1 + X, kGroupWarps * 32);
+          if (gt < R) {
+            const float top = fmaxf(fmaxf(S.part_max[X][0][gt], S.part_max[X][1][gt]),
+                                    fmaxf(S.part_max[X][2][gt], S.part_max[X][3][gt])) - kOff;
+            const float old = S.ref[X][gt], now = top > old + kLazy ? top : old;
+            S.ref[X][gt] = now;
+            S.alpha[X][gt] = ex2(old - now);
+          }
+          named_bar_sync(1 + X, kGroupWarps * 32);
+#pragma unroll
+          for (int r = 0; r < R; ++r) l[r] *= S.alpha[X][r];
+          if (j > first) {
+#pragma unroll
+            for (int c = 0; c < R / CH; ++c) {
+              float hi[CH], lo[CH];
+              tc::ld_wait(t_o + CH * c, t_o + R + CH * c, hi, lo);
+#pragma unroll
+              for (int r = 0; r < CH; ++r) {
+                hi[r] *= S.alpha[X][CH * c + r];
+                lo[r] *= S.alpha[X][CH * c + r];
+              }
+              tc::st(t_o + CH * c, hi);
+              tc::st(t_o + R + CH * c, lo);
+            }
+            tc::wait_st();
+          }
         }
 #pragma unroll
         for (int c = 0; c < R / CH; ++c) {
-          if constexpr (R > CH) {
-            scores(c);
-            reference(c, false);
-          }
+          float* y = kKeep ? x + CH * c : x;
+          if constexpr (!kKeep) scores(c, y);
+          float m[CH];
+          row_values(m, S.ref[X] + CH * c);
+          uint32_t h[CH / 4], g[CH / 4];
 #pragma unroll
-          for (int r = 0; r < CH; ++r) {
-            const int a = CH * c + r;
-            const float pr = ex2(x[r] - (m[r] == -INFINITY ? 0.f : m[r] - kOff));
-            l[a] = fmaf(pr, inv_vs, l[a]);
-            float hi, lo;
-            split4(pr, hi, lo);
-            const uint32_t b = e4m3x2(hi, lo * kLo);
-            sp[swz(a, gt >> 4) + (gt & 15)] = (uint8_t)b;
-            sp[swz(R + a, gt >> 4) + (gt & 15)] = (uint8_t)(b >> 8);
+          for (int r = 0; r < CH; r += 4) {
+            float hi[4], lo[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int a = CH * c + r + u;
+              const float pr = ex2(y[r + u] - m[r + u]);
+              l[a] = fmaf(pr, inv_vs, l[a]);
+              split4(pr, hi[u], lo[u]);
+            }
+            h[r / 4] = e4m3x2(hi[0], hi[1]) | (e4m3x2(hi[2], hi[3]) << 16);
+            g[r / 4] = e4m3x2(lo[0] * kLo, lo[1] * kLo) | (e4m3x2(lo[2] * kLo, lo[3] * kLo) << 16);
+          }
+          if constexpr (R == 8) {
+            *reinterpret_cast<uint4*>(sp + SH::p_at(gt, 0)) = make_uint4(h[0], h[1], g[0], g[1]);
+          } else {
+            *reinterpret_cast<uint4*>(sp + SH::p_at(gt, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(sp + SH::p_at(gt, R / 16 + c)) = make_uint4(g[0], g[1], g[2], g[3]);
           }
         }
+        if constexpr (!kKeep) release();
         if (!seen) {
           uint4* v = reinterpret_cast<uint4*>(smem + st * 2 * kHalf + kHalf + gt * kHead);
 #pragma unroll
@@ -530,16 +592,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane == (r & 31)) S.fin_l[X][gw][r] = v;
       }
-      if (gt < R) S.fin_m[X][gt] = own > 0 ? S.ref[X][(klast & 1) ^ 1][gt] : -INFINITY;
+      if (gt < R) S.fin_m[X][gt] = S.ref[X][gt];  // kNone where the group had no tile
       named_bar_sync(3, kSoftWarps * 32);
       auto weight = [&](int g, int r) {  // of group g in row r's sum
-        const float a = S.fin_m[g][r], b = S.fin_m[g ^ 1][r];
-        return a == -INFINITY ? 0.f : ex2(a - fmaxf(a, b));
+        return ex2(S.fin_m[g][r] - fmaxf(S.fin_m[g][r], S.fin_m[g ^ 1][r]));
       };
       auto output = [&](int c, float (&o)[CH]) {  // this group's O^T of rows CH c .., dimension gt
         float lo[CH];
-        tc::ld_wait(t_o + CH * c, o);
-        tc::ld_wait(t_o + R + CH * c, lo);
+        tc::ld_wait(t_o + CH * c, t_o + R + CH * c, o, lo);
 #pragma unroll
         for (int r = 0; r < CH; ++r) o[r] = fmaf(lo[r], 1.f / kLo, o[r]) * weight(X, CH * c + r);
       };
@@ -572,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int t = a / p.group;
         const __nv_bfloat162 u = __floats2bfloat162_rn(o.x * f, o.y * f), v = __floats2bfloat162_rn(o.z * f, o.w * f);
         *reinterpret_cast<uint2*>(p.out + (int64_t)(s.row0 + t) * p.o_st +
-                                  (int64_t)(w.kh * p.group + a - t * p.group) * p.o_sh + 4 * c) =
+                                  (int64_t)(kh * p.group + a - t * p.group) * p.o_sh + 4 * c) =
             make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
       };
       const bool whole = n == s.tiles;
@@ -597,9 +657,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!whole) {
         __threadfence();
         named_bar_sync(3, kSoftWarps * 32);
-        const int c_lo = share_owner(w.item, total, ctas), c_hi = share_owner(w.item + s.tiles - 1, total, ctas);
+        const int c_lo = share_owner(w.item, total, shares), c_hi = share_owner(w.item + s.tiles - 1, total, shares);
         if (tid == 0) {
-          int* counter = p.counters + (int64_t)w.seq * p.hkv + w.kh;
+          int* counter = p.counters + (int64_t)w.seq * p.hkv + kh;
           S.last = atomicAdd(counter, 1) == c_hi - c_lo;
           if (S.last) *counter = 0;
         }
@@ -608,10 +668,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           __threadfence();
           // the shares of the item in order, kJoin loads of each kind in flight
           constexpr int kJoin = 8;
-          const int slot0 = 2 * c_lo + (w.item >= share_begin(c_lo, total, ctas) ? 1 : 0);  // later ones begin inside it
+          // later shares begin inside the item: it is their first
+          const int at0 = w.item >= share_begin(c_lo, total, shares) ? 1 : 0;
           for (int e = tid; e < rows * (kHead / 4); e += kSoftWarps * 32) {
             const int a = e / (kHead / 4), c = e % (kHead / 4);
-            float top = -INFINITY, sum = 0.f;
+            float top = kNone, sum = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int c0 = c_lo; c0 <= c_hi; c0 += kJoin) {
               float2 ml[kJoin];
@@ -619,27 +680,27 @@ __global__ void __launch_bounds__(kThreads, 1)
               float nt = top;
 #pragma unroll
               for (int u = 0; u < kJoin; ++u) {
-                ml[u] = make_float2(-INFINITY, 0.f);
+                ml[u] = make_float2(kNone, 0.f);
+                v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (c0 + u <= c_hi) {
-                  const float* q = p.partials + (int64_t)(c0 + u == c_lo ? slot0 : 2 * (c0 + u)) * kPart;
+                  const int64_t cta = (int64_t)(c0 + u) * p.slots + slot;
+                  const float* q = p.partials + (2 * cta + (c0 + u == c_lo ? at0 : 0)) * kPart;
                   ml[u] = __ldcg(reinterpret_cast<const float2*>(q + kMaxRows * kHead + 2 * a));
                   v[u] = __ldcg(reinterpret_cast<const float4*>(q + a * kHead + 4 * c));
                 }
               }
 #pragma unroll
               for (int u = 0; u < kJoin; ++u) nt = fmaxf(nt, ml[u].x);
-              if (nt == -INFINITY) continue;
               const float f = ex2(top - nt);
               sum *= f;
               o.x *= f; o.y *= f; o.z *= f; o.w *= f;
 #pragma unroll
-              for (int u = 0; u < kJoin; ++u)
-                if (ml[u].x != -INFINITY) {
-                  const float g = ex2(ml[u].x - nt);
-                  sum = fmaf(g, ml[u].y, sum);
-                  o.x = fmaf(g, v[u].x, o.x); o.y = fmaf(g, v[u].y, o.y);
-                  o.z = fmaf(g, v[u].z, o.z); o.w = fmaf(g, v[u].w, o.w);
-                }
+              for (int u = 0; u < kJoin; ++u) {
+                const float g = ex2(ml[u].x - nt);
+                sum = fmaf(g, ml[u].y, sum);
+                o.x = fmaf(g, v[u].x, o.x); o.y = fmaf(g, v[u].y, o.y);
+                o.z = fmaf(g, v[u].z, o.z); o.w = fmaf(g, v[u].w, o.w);
+              }
               top = nt;
             }
             store(a, c, o, sum);
@@ -652,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == kSoftWarps + 1) tc::tmem_dealloc(tbase, SH::kTmem);
+  if (warp == kQkWarp) tc::tmem_dealloc(tbase, SH::kTmem);
 }
 
 template <int R>
@@ -676,9 +737,21 @@ cudaError_t launch(const CUtensorMap& km, const CUtensorMap& vm, const BlockAttn
 
 }  // namespace
 
-cudaError_t block_decode_launch(const CUtensorMap& km, const CUtensorMap& vm, const BlockAttnParams& p, int rows,
+cudaError_t block_decode_launch(const CUtensorMap& km, const CUtensorMap& vm, BlockAttnParams p, int rows,
                                 cudaStream_t st) {
-  const int ctas = num_sms_current_device() < kMaxCtas ? num_sms_current_device() : kMaxCtas;
+  // kv heads walked by one CTA, one after the other: the fewest that keep the most
+  // SMs busy (8 heads: one each on 18 x 8 = 144 of 148 SMs)
+  const int sms = num_sms_current_device() < kMaxCtas ? num_sms_current_device() : kMaxCtas;
+  int ctas = 0;
+  for (int heads = 1; heads <= p.hkv; ++heads) {
+    if (p.hkv % heads) continue;
+    const int slots = p.hkv / heads, n = sms / slots * slots;
+    if (n > ctas + ctas / 16) {
+      ctas = n;
+      p.heads = heads;
+      p.slots = slots;
+    }
+  }
   if (rows <= 8) return launch<8>(km, vm, p, ctas, st);
   if (rows <= 16) return launch<16>(km, vm, p, ctas, st);
   if (rows <= 32) return launch<32>(km, vm, p, ctas, st);
