@@ -397,11 +397,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* join = reinterpret_cast<float*>(smem + SH::kOffP);  // [R][kHead]
     bool failed = false;
     int i0 = 0, seg = 0;
-    for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0; w.next(), ++seg) {
-      const int n = w.count(), qb = seg & 1, kh = w.kh();
-      const Span& s = w.s;
+    // Q of a segment, with its rows' factors and positions: a power-of-two prescale
+    // per row (maximum in [2^7, 2^8)), two terms
+    auto put_q = [&](const Span& s, int kh, int qb) {
       const int rows = s.qlen * p.group;
-      // ---- Q: per-row power-of-two prescale (maximum in [2^7, 2^8)), two terms -----------
       for (int e = tid; e < R * 8; e += kSoftWarps * 32) {
         const int r = e >> 3, c = e & 7, t = r / p.group;
         uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
@@ -443,6 +442,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&S.q_full[qb]);
+    };
+    Walk w(p, R, S.first_seq, S.first_prefix, begin, count);
+    put_q(w.s, w.kh(), 0);
+    for (; w.left > 0; ++seg) {
+      const int n = w.count(), qb = seg & 1, kh = w.kh(), seq = w.seq;
+      const Span s = w.s;
+      const int64_t item = w.item;
+      const int off = w.off, rows = s.qlen * p.group;
+      // the next segment's Q goes out now, so that its first product need not wait for
+      // this one's end (the buffer's last reader ended with the segment before)
+      w.next();
+      if (w.left > 0) put_q(w.s, w.kh(), qb ^ 1);
       if (gt < R) S.ref[X][gt] = kNone;
       named_bar_sync(3, kSoftWarps * 32);  // factor, pos and ref are visible
 
@@ -452,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int first = (i0 ^ X) & 1;  // the segment's first tile of this group
       for (int j = first; j < n; j += 2) {
         const int i = i0 + j, st = i % NS, k = i >> 1;  // k: the group's tiles so far
-        const int key0 = s.tile(w.off + j) * kTile, key = key0 + gt;
+        const int key0 = s.tile(off + j) * kTile, key = key0 + gt;
         const uint32_t t_s = tbase + (i % LK) * N + lane_off;
         if (!failed) failed = !mbar_wait_bounded(&S.s_full[i % LK], (i / LK) & 1);
         tc::fence_after_sync();
@@ -475,9 +486,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           float f[CH];
           row_values(f, S.factor[qb] + CH * c);
 #pragma unroll
-          for (int r = 0; r < CH; ++r) {
-            y[r] = fmaf(fmaf(lo[r], 1.f / kLo, hi[r]) * f[r], ks, lvs);
-            if (!open) {
+          for (int r = 0; r < CH; ++r) y[r] = fmaf(fmaf(lo[r], 1.f / kLo, hi[r]) * f[r], ks, lvs);
+          if (!open) {  // few tiles: a branch around all rows keeps the others' code short
+#pragma unroll
+            for (int r = 0; r < CH; ++r) {
               const int pos = S.pos[qb][CH * c + r];
               if (!(seen && key <= pos && (p.window == 0 || key > pos - p.window || key < p.sinks))) y[r] = kMasked;
             }
@@ -637,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       const bool whole = n == s.tiles;
       constexpr int kPart = kMaxRows * (kHead + 2);
-      float* part = p.partials + (int64_t)(2 * blockIdx.x + (w.item >= begin ? 1 : 0)) * kPart;
+      float* part = p.partials + (int64_t)(2 * blockIdx.x + (item >= begin ? 1 : 0)) * kPart;
       for (int e = tid; e < rows * (kHead / 4); e += kSoftWarps * 32) {
         const int a = e / (kHead / 4), c = e % (kHead / 4);
         const float4 o = *reinterpret_cast<const float4*>(join + a * kHead + 4 * c);
@@ -657,9 +669,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!whole) {
         __threadfence();
         named_bar_sync(3, kSoftWarps * 32);
-        const int c_lo = share_owner(w.item, total, shares), c_hi = share_owner(w.item + s.tiles - 1, total, shares);
+        const int c_lo = share_owner(item, total, shares), c_hi = share_owner(item + s.tiles - 1, total, shares);
         if (tid == 0) {
-          int* counter = p.counters + (int64_t)w.seq * p.hkv + kh;
+          int* counter = p.counters + (int64_t)seq * p.hkv + kh;
           S.last = atomicAdd(counter, 1) == c_hi - c_lo;
           if (S.last) *counter = 0;
         }
@@ -669,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // the shares of the item in order, kJoin loads of each kind in flight
           constexpr int kJoin = 8;
           // later shares begin inside the item: it is their first
-          const int at0 = w.item >= share_begin(c_lo, total, shares) ? 1 : 0;
+          const int at0 = item >= share_begin(c_lo, total, shares) ? 1 : 0;
           for (int e = tid; e < rows * (kHead / 4); e += kSoftWarps * 32) {
             const int a = e / (kHead / 4), c = e % (kHead / 4);
             float top = kNone, sum = 0.f;
