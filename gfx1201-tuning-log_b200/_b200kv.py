@@ -12,6 +12,7 @@ Entry points mirror include/b200kv.h; every call returns a status that
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("B200KV_LIB", os.path.join(_HERE, "libb200kv.so"))
@@ -158,32 +159,18 @@ lib.b200kv_kv_write.argtypes = ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp] + [
                                 [_vp, _vp, _vp] + [_i32] * 5 + [_vp])
 
 
-class BlockCacheDesc(ctypes.Structure):
-    """b200kv_block_cache (include/b200kv.h)."""
-    _fields_ = ([(n, _vp) for n in ("k", "v", "k_scales", "v_scales", "block_table")] +
-                [(n, _i64) for n in ("sk0", "sk1", "sk2", "sv0", "sv1", "sv2", "ks0", "ks1", "vs0", "vs1",
-                                     "bt_stride")] +
-                [(n, ctypes.c_int32) for n in ("num_blocks", "block_size", "num_kv_heads", "head_dim",
-                                               "max_blocks", "num_seqs")])
-
-
-class BlockAttnArgs(ctypes.Structure):
-    """b200kv_block_attn_args (include/b200kv.h)."""
-    _fields_ = ([(n, _vp) for n in ("q", "out", "cu_seqlens_q", "seq_lens", "workspace")] +
-                [("workspace_bytes", ctypes.c_size_t)] +
-                [(n, _i64) for n in ("q_stride_tok", "q_stride_head", "out_stride_tok", "out_stride_head")] +
-                [("sm_scale", _f32)] +
-                [(n, ctypes.c_int32) for n in ("num_tokens", "max_qlen", "max_seq_len", "num_q_heads", "window",
-                                               "sinks", "reserved")])
-
+# b200kv_block_cache and b200kv_block_attn_args (include/b200kv.h), packed in one
+# go: a call of a few microseconds pays for every field of a ctypes.Structure
+BLOCK_CACHE = struct.Struct("@5P11q6i")  # k, v, k_scales, v_scales, block_table; sk0 .. bt_stride; num_blocks ..
+BLOCK_ATTN_ARGS = struct.Struct("@5PN4qf7i")  # q, out, cu, lens, workspace; its bytes; strides; sm_scale; num_tokens ..
 
 lib.b200kv_block_append.restype = _i32
-lib.b200kv_block_append.argtypes = [ctypes.POINTER(BlockCacheDesc), _vp, _i64, _vp, _i32, _vp, _i64, _i64, _vp, _vp,
+lib.b200kv_block_append.argtypes = [ctypes.c_char_p, _vp, _i64, _vp, _i32, _vp, _i64, _i64, _vp, _vp,
                                     _i32, _i32, _vp]
 lib.b200kv_block_attn_workspace_bytes.restype = ctypes.c_size_t
 lib.b200kv_block_attn_workspace_bytes.argtypes = [_i32, _i32]
 lib.b200kv_block_attn.restype = _i32
-lib.b200kv_block_attn.argtypes = [ctypes.POINTER(BlockCacheDesc), ctypes.POINTER(BlockAttnArgs), _vp]
+lib.b200kv_block_attn.argtypes = [ctypes.c_char_p, ctypes.c_char_p, _vp]
 lib.b200kv_spec_verify.restype = _i32
 lib.b200kv_spec_verify.argtypes = [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _i32,
                                    _i32, _vp]

@@ -12,45 +12,47 @@ float32 [NB, HKV]: a code stands for code * scale.  Sequence s keeps token p at
 block block_table[s, p // BS], slot p % BS.  Neither call reads the host's copy
 of a length, so both can be captured in CUDA graphs.
 """
-import ctypes
-
 import torch
 
-from _b200kv import BlockAttnArgs, BlockCacheDesc, check, lib
+from _b200kv import BLOCK_ATTN_ARGS, BLOCK_CACHE, check, lib
 
 HEAD_DIM = 128
-_FP8 = torch.float8_e4m3fn
+_FP8, _BF16, _F32, _I32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32, torch.int32
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _describe(k_cache, v_cache, k_scales, v_scales, block_table):
-    if k_cache.dtype != _FP8 or v_cache.dtype != _FP8:
+def _describe(k_cache, v_cache, k_scales, v_scales, block_table, cu_seqlens, seq_lens):
+    """The packed b200kv_block_cache, kv heads and sequences of checked tensors.
+    (Plain attribute reads in one place: a decoding step makes these calls once a
+    layer, and each costs the host about as long as the kernel runs.)"""
+    if k_cache.dtype is not _FP8 or v_cache.dtype is not _FP8:
         raise TypeError("k_cache and v_cache must be float8_e4m3fn")
-    if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
+    if k_scales.dtype is not _F32 or v_scales.dtype is not _F32:
         raise TypeError("k_scales and v_scales must be float32")
-    if block_table.dtype != torch.int32:
-        raise TypeError("block_table must be int32")
-    nb, bs, hkv, d = k_cache.shape
-    if v_cache.shape != k_cache.shape:
+    if block_table.dtype is not _I32 or cu_seqlens.dtype is not _I32 or seq_lens.dtype is not _I32:
+        raise TypeError("block_table, cu_seqlens and seq_lens must be int32")
+    shape = k_cache.shape
+    nb, bs, hkv, d = shape
+    if v_cache.shape != shape:
         raise ValueError("k_cache and v_cache shapes differ")
     if k_scales.shape != (nb, hkv) or v_scales.shape != (nb, hkv):
         raise ValueError(f"k_scales and v_scales must be [{nb}, {hkv}]")
-    sk, sv, bt = k_cache.stride(), v_cache.stride(), block_table.stride()
-    if sk[3] != 1 or sv[3] != 1 or bt[1] != 1:
-        raise ValueError("k_cache, v_cache and block_table must have unit innermost stride")
     seqs, blocks = block_table.shape
-    ks, vs = k_scales.stride(), v_scales.stride()
-    return BlockCacheDesc(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
-                          block_table.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], ks[0], ks[1], vs[0],
-                          vs[1], bt[0], nb, bs, hkv, d, blocks, seqs)
-
-
-def _batch(cu_seqlens, seq_lens, seqs):
-    if cu_seqlens.dtype != torch.int32 or seq_lens.dtype != torch.int32:
-        raise TypeError("cu_seqlens and seq_lens must be int32")
     if cu_seqlens.shape != (seqs + 1,) or seq_lens.shape != (seqs,):
         raise ValueError(f"cu_seqlens must be [{seqs + 1}] and seq_lens [{seqs}], as block_table has rows")
     if not (cu_seqlens.is_contiguous() and seq_lens.is_contiguous()):
         raise ValueError("cu_seqlens and seq_lens must be contiguous")
+    sk0, sk1, sk2, sk3 = k_cache.stride()
+    sv0, sv1, sv2, sv3 = v_cache.stride()
+    bt0, bt1 = block_table.stride()
+    if sk3 != 1 or sv3 != 1 or bt1 != 1:
+        raise ValueError("k_cache, v_cache and block_table must have unit innermost stride")
+    ks0, ks1 = k_scales.stride()
+    vs0, vs1 = v_scales.stride()
+    desc = BLOCK_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                            block_table.data_ptr(), sk0, sk1, sk2, sv0, sv1, sv2, ks0, ks1, vs0, vs1, bt0, nb, bs, hkv,
+                            d, blocks, seqs)
+    return desc, hkv, seqs
 
 
 def append(qkv, cos_sin, k_cache, v_cache, k_scales, v_scales, cu_seqlens, seq_lens, block_table, q_out=None):
@@ -64,28 +66,31 @@ def append(qkv, cos_sin, k_cache, v_cache, k_scales, v_scales, cu_seqlens, seq_l
     values (x / scale within e4m3's 448); a block that outgrows it has its earlier
     codes rounded again.  Two sequences may not append to one block.
     """
-    if qkv.dtype != torch.bfloat16:
+    if qkv.dtype is not _BF16:
         raise TypeError("qkv must be bfloat16")
-    if cos_sin.dtype != torch.float32:
+    if cos_sin.dtype is not _F32:
         raise TypeError("cos_sin must be float32")
-    desc = _describe(k_cache, v_cache, k_scales, v_scales, block_table)
-    _batch(cu_seqlens, seq_lens, desc.num_seqs)
+    desc, hkv, _ = _describe(k_cache, v_cache, k_scales, v_scales, block_table, cu_seqlens, seq_lens)
     tokens, width = qkv.shape
-    hq = width // HEAD_DIM - 2 * desc.num_kv_heads
-    if width % HEAD_DIM or hq <= 0 or hq % desc.num_kv_heads:
-        raise ValueError(f"qkv rows of {width} are not [q | k | v] heads of {HEAD_DIM} over {desc.num_kv_heads} kv heads")
-    if cos_sin.dim() != 2 or cos_sin.shape[1] != HEAD_DIM or not cos_sin.is_contiguous() or qkv.stride(1) != 1:
+    hq = width // HEAD_DIM - 2 * hkv
+    if width % HEAD_DIM or hq <= 0 or hq % hkv:
+        raise ValueError(f"qkv rows of {width} are not [q | k | v] heads of {HEAD_DIM} over {hkv} kv heads")
+    positions, d = cos_sin.shape
+    row, one = qkv.stride()
+    if d != HEAD_DIM or not cos_sin.is_contiguous() or one != 1:
         raise ValueError("cos_sin must be contiguous [max_pos, 128] and qkv rows contiguous")
     if q_out is None:
         q_out = qkv[:, :hq * HEAD_DIM].unflatten(1, (hq, HEAD_DIM))
-    elif q_out.dtype != torch.bfloat16:
+    elif q_out.dtype is not _BF16:
         raise TypeError("q_out must be bfloat16")
-    if q_out.shape != (tokens, hq, HEAD_DIM) or q_out.stride(2) != 1:
+    q0, q1, q2 = q_out.stride()
+    if q_out.shape != (tokens, hq, HEAD_DIM) or q2 != 1:
         raise ValueError(f"q_out must be [{tokens}, {hq}, {HEAD_DIM}] with unit innermost stride")
-    check(lib.b200kv_block_append(
-        ctypes.byref(desc), qkv.data_ptr(), qkv.stride(0), cos_sin.data_ptr(), cos_sin.shape[0], q_out.data_ptr(),
-        q_out.stride(0), q_out.stride(1), cu_seqlens.data_ptr(), seq_lens.data_ptr(), tokens, hq,
-        torch.cuda.current_stream(qkv.device).cuda_stream), "b200kv_block_append")
+    status = lib.b200kv_block_append(desc, qkv.data_ptr(), row, cos_sin.data_ptr(), positions, q_out.data_ptr(), q0, q1,
+                                     cu_seqlens.data_ptr(), seq_lens.data_ptr(), tokens, hq,
+                                     _raw_stream(qkv.device.index))
+    if status:
+        check(status, "b200kv_block_append")
     return q_out
 
 
@@ -99,6 +104,7 @@ class Workspace:
         self.num_seqs, self.num_kv_heads = num_seqs, num_kv_heads
         self.buffer = torch.zeros(lib.b200kv_block_attn_workspace_bytes(num_seqs, num_kv_heads), dtype=torch.uint8,
                                   device=device)
+        self.pointer, self.bytes = self.buffer.data_ptr(), self.buffer.numel()
 
 
 def attention(q, k_cache, v_cache, k_scales, v_scales, out, cu_seqlens_q, seq_lens, block_table, sm_scale, max_qlen,
@@ -112,23 +118,24 @@ def attention(q, k_cache, v_cache, k_scales, v_scales, out, cu_seqlens_q, seq_le
     (0: what block_table holds) bound the batch's query counts and lengths.
     workspace: a Workspace, or None for one made for this call.
     """
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+    if q.dtype is not _BF16 or out.dtype is not _BF16:
         raise TypeError("q and out must be bfloat16")
-    desc = _describe(k_cache, v_cache, k_scales, v_scales, block_table)
-    _batch(cu_seqlens_q, seq_lens, desc.num_seqs)
-    if q.dim() != 3 or q.shape[2] != HEAD_DIM or out.shape != q.shape:
+    desc, hkv, seqs = _describe(k_cache, v_cache, k_scales, v_scales, block_table, cu_seqlens_q, seq_lens)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != HEAD_DIM or out.shape != shape:
         raise ValueError(f"q and out must be [tokens, heads, {HEAD_DIM}]")
-    sq, so = q.stride(), out.stride()
-    if sq[2] != 1 or so[2] != 1:
+    q0, q1, q2 = q.stride()
+    o0, o1, o2 = out.stride()
+    if q2 != 1 or o2 != 1:
         raise ValueError("q and out must have unit innermost stride")
     if workspace is None:
-        workspace = Workspace(q.device, desc.num_seqs, desc.num_kv_heads)
-    elif workspace.num_seqs < desc.num_seqs or workspace.num_kv_heads < desc.num_kv_heads:
+        workspace = Workspace(q.device, seqs, hkv)
+    elif workspace.num_seqs < seqs or workspace.num_kv_heads < hkv:
         raise ValueError("workspace is for fewer sequences or kv heads")
-    ws = workspace.buffer
-    args = BlockAttnArgs(q.data_ptr(), out.data_ptr(), cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), ws.data_ptr(),
-                         ws.numel(), sq[0], sq[1], so[0], so[1], sm_scale, q.shape[0], max_qlen,
-                         max_seq_len or desc.max_blocks * desc.block_size, q.shape[1], window, sinks, 0)
-    check(lib.b200kv_block_attn(ctypes.byref(desc), ctypes.byref(args),
-                                torch.cuda.current_stream(q.device).cuda_stream), "b200kv_block_attn")
+    args = BLOCK_ATTN_ARGS.pack(q.data_ptr(), out.data_ptr(), cu_seqlens_q.data_ptr(), seq_lens.data_ptr(),
+                                workspace.pointer, workspace.bytes, q0, q1, o0, o1, sm_scale, shape[0], max_qlen,
+                                max_seq_len or block_table.shape[1] * k_cache.shape[1], shape[1], window, sinks, 0)
+    status = lib.b200kv_block_attn(desc, args, _raw_stream(q.device.index))
+    if status:
+        check(status, "b200kv_block_attn")
     return out

@@ -6,11 +6,34 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace b200kv {
 
 constexpr int kMaxGroup = 16;  // query heads per kv head
 constexpr int kMaxRows = 64;   // (query token, head) rows of a kv head that the few-query kernel takes
 constexpr int kMaxCtas = 160;  // shares of a batch it is cut into, at most
+
+// Whether something was done once on the current device (a kernel's attribute set).
+class PerDevice {
+ public:
+  bool done() const {
+    const int d = device();
+    return d >= 0 && done_[d].load(std::memory_order_acquire);
+  }
+  void set() {
+    const int d = device();
+    if (d >= 0) done_[d].store(true, std::memory_order_release);
+  }
+
+ private:
+  static constexpr int kDevices = 64;
+  static int device() {
+    int d = -1;
+    return cudaGetDevice(&d) == cudaSuccess && d < kDevices ? d : -1;
+  }
+  std::atomic<bool> done_[kDevices] = {};
+};
 
 struct BlockAttnParams {
   const __nv_bfloat16* q;

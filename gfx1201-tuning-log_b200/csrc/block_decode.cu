@@ -25,8 +25,8 @@
 // item to finish (a counter, back at zero afterwards) joins them in order, so the
 // sum does not depend on who is last.
 //
-// Roles: 8 softmax warps in two groups that take alternate tiles (own O, P and
-// running state each, joined at the item's end), a TMA warp for K and one for V, a
+// Roles: softmax warps in two groups that take alternate tiles (own O, P and
+// running state each, joined at the item's end; one group for 64 rows), a TMA warp for K and one for V, a
 // warp that issues the first product and one that issues the second (a thread
 // issues an MMA in about 100 cycles: one issuer for all eight of a tile, or one TMA
 // warp for its sixteen 2 KB pages, bounds the kernel).
@@ -55,11 +55,7 @@ namespace {
 constexpr int kHead = 128;
 constexpr int kTile = 128;                  // keys per tile
 constexpr int kHalf = kTile * kHead;        // K (or V) bytes of a tile
-constexpr int kGroupWarps = 4;
-constexpr int kSoftWarps = 2 * kGroupWarps;
-constexpr int kQkWarp = kSoftWarps, kPvWarp = kSoftWarps + 1, kTmaWarp = kSoftWarps + 2;  // K's, then V's
-constexpr int kWarps = kSoftWarps + 4;
-constexpr int kThreads = kWarps * 32;
+constexpr int kPart = kMaxRows * (kHead + 2);  // floats of a partial: o, then (m, l) of each row
 constexpr int kMaxPages = 8;                // pages per tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 4.f;                // the reference moves when a maximum exceeds it by 2^4
@@ -72,15 +68,26 @@ constexpr float kNone = -1e30f;             // the reference of a row that has s
 
 template <int R>
 struct Shape {
+  // rows of a softmax thread; warps of a group: four quadrants of 32 keys for each
+  // kRows rows, so that scores and sums stay in registers
+  static constexpr int kRows = R < 16 ? R : 16;
+  static constexpr int kParts = R / kRows;
+  static constexpr int kGroups = R < 64 ? 2 : 1;
+  static constexpr int kGroupWarps = 4 * kParts;
+  static constexpr int kSoftWarps = kGroups * kGroupWarps;
+  static constexpr int kQkWarp = kSoftWarps, kPvWarp = kSoftWarps + 1, kTmaWarp = kSoftWarps + 2;  // K's, V's
+  static constexpr int kWarps = kSoftWarps + 4;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kN = 2 * R;          // columns of S^T and O^T: hi rows, lo rows
   static constexpr int kStages = R >= 64 ? 4 : R == 32 ? 5 : 6;
+  static constexpr int kLook = R >= 64 ? 2 : 4;      // score tiles in tensor memory
+  static constexpr uint32_t kTmem = R == 8 ? 128 : R == 16 ? 256 : 512;  // kLook S and kGroups O tiles of N columns
   static constexpr int kOperand = kN * 128; // bytes of Q or P
   static constexpr int kOffQ = kStages * 2 * kHalf;  // [segment parity]
   static constexpr int kOffP = kOffQ + 2 * kOperand; // [group][key][N]; the groups' join at a segment's end
-  static constexpr int kBytes = kOffP + 2 * kOperand;
-  static constexpr int kChunk = R < 16 ? R : 16;     // rows handled together
-  static constexpr int kLook = R >= 64 ? 2 : 4;      // score tiles in tensor memory
-  static constexpr uint32_t kTmem = R == 8 ? 128 : R == 16 ? 256 : 512;  // kLook S + 2 O tiles of N columns
+  static constexpr int kBytes = kOffP + R * kHead * 4;
+  static_assert((kLook + kGroups) * kN <= (int)kTmem && kStages > kLook && kGroups * kOperand <= R * kHead * 4,
+                "tensor memory; a stage free to load into; P fits where the join goes");
   // P rows of N bytes, swizzled over their width (none, 32, 64, 128 bytes)
   static constexpr uint32_t kLayoutP = R == 8 ? 0 : R == 16 ? 6 : R == 32 ? 4 : 2;
   __device__ static __forceinline__ uint32_t p_at(int key, int chunk) {
@@ -89,7 +96,6 @@ struct Shape {
   __device__ static __forceinline__ uint64_t p_desc(uint32_t addr) {  // 8-key groups 8 N bytes apart
     return R == 8 ? tc::sdesc(addr, 8 * kN, 16, kLayoutP) : tc::sdesc(addr, 16, 8 * kN, kLayoutP);
   }
-  static_assert((kLook + 2) * kN <= (int)kTmem && kStages > kLook, "tensor memory; a stage free to load into");
 };
 
 template <int R>
@@ -100,12 +106,12 @@ struct Shared {
   float scale[Shape<R>::kStages][2][kMaxPages];      // ks, vs of a tile's pages
   alignas(16) float factor[2][R];                    // [segment parity] score factor of a row
   alignas(16) int pos[2][R];                         // and its position
-  alignas(16) float part_max[2][kGroupWarps][R];     // [group][warp]
+  alignas(16) float part_max[2][4][R];               // [group][quadrant]
   alignas(16) float ref[2][R];                       // [group] P = 2^(x - ref)
   alignas(16) float alpha[2][R];                     // and what its last move scales O and l by
-  alignas(16) float fin_m[2][R], fin_l[2][kGroupWarps][R];
+  alignas(16) float fin_m[2][R], fin_l[2][4][R];
   int first_seq, first_prefix, last;
-  int warp_sum[kWarps];
+  int warp_sum[Shape<R>::kWarps];
 };
 
 // CH per-row values from shared memory (16-byte aligned)
@@ -204,11 +210,13 @@ __device__ __forceinline__ int share_owner(int64_t tile, int64_t total, int64_t 
 }
 
 template <int R>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<R>::kThreads, 1)
     block_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                         const BlockAttnParams p) {
   using SH = Shape<R>;
-  constexpr int N = SH::kN, NS = SH::kStages, CH = SH::kChunk, LK = SH::kLook;
+  constexpr int N = SH::kN, NS = SH::kStages, LK = SH::kLook, G = SH::kGroups, RT = SH::kRows;
+  constexpr int CH = R == 16 ? 16 : 8;  // rows read together: 16 where the registers allow it
+  constexpr int kThreads = SH::kThreads, kSoftThreads = SH::kSoftWarps * 32;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ Shared<R> S;
@@ -221,17 +229,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&S.kv_empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&S.q_full[b], kSoftWarps);
-      mbar_init(&S.p_full[b], kGroupWarps);
+      mbar_init(&S.q_full[b], SH::kSoftWarps);
+      mbar_init(&S.p_full[b], SH::kGroupWarps);
       mbar_init(&S.pv_done[b], 1);
     }
     for (int b = 0; b < LK; ++b) {
       mbar_init(&S.s_full[b], 1);
-      mbar_init(&S.s_free[b], kGroupWarps);
+      mbar_init(&S.s_free[b], SH::kGroupWarps);
     }
     fence_mbar_init();
   }
-  if (warp == kQkWarp) tc::tmem_alloc(&S.tmem, SH::kTmem);
+  if (warp == SH::kQkWarp) tc::tmem_alloc(&S.tmem, SH::kTmem);
   griddep_wait();  // lengths, tables and q may be the previous kernel's
 
   // ---- this CTA's share: an inclusive scan of the sequences' tile counts -------------
@@ -251,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after_sync();
   int before = 0, tiles = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < SH::kWarps; ++w) {
     if (w < warp) before += S.warp_sum[w];
     tiles += S.warp_sum[w];
   }
@@ -274,22 +282,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         at += n;
       }
   }
-  // queries of sequences without a key: zeros
-  for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
-    const Span sp = span_of(p, s, R);
-    if (sp.tiles == 0 && sp.qlen > 0 && sp.qlen <= R && sp.qlen * p.group <= R)
-      for (int i = tid; i < sp.qlen * p.hkv * p.group * kHead; i += kThreads) {
-        const int t = i / (p.hkv * p.group * kHead), h = i / kHead % (p.hkv * p.group);
-        p.out[(int64_t)(sp.row0 + t) * p.o_st + (int64_t)h * p.o_sh + i % kHead] = __float2bfloat16_rn(0.f);
-      }
-  }
   __syncthreads();
   const uint32_t tbase = S.tmem;  // LK score tiles, O of group 0 and 1: N columns each
 
+  if (warp == SH::kPvWarp) {  // it waits for the first P anyway
+    // queries of sequences without a key: zeros
+    for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
+      const Span sp = span_of(p, s, R);
+      if (sp.tiles == 0 && sp.qlen > 0 && sp.qlen <= R && sp.qlen * p.group <= R)
+        for (int i = lane; i < sp.qlen * p.hkv * p.group * kHead; i += 32) {
+          const int t = i / (p.hkv * p.group * kHead), h = i / kHead % (p.hkv * p.group);
+          p.out[(int64_t)(sp.row0 + t) * p.o_st + (int64_t)h * p.o_sh + i % kHead] = __float2bfloat16_rn(0.f);
+        }
+    }
+  }
   if (!busy) {
-  } else if (warp >= kTmaWarp) {
+  } else if (warp >= SH::kTmaWarp) {
     // ---------------- TMA producers: K pages, V pages -----------------------------------
-    const bool is_v = warp > kTmaWarp;
+    const bool is_v = warp > SH::kTmaWarp;
     const CUtensorMap* map = is_v ? &vmap : &kmap;
     const float* scales = is_v ? p.vs : p.ks;
     const int64_t sc0 = is_v ? p.vs0 : p.ks0, sc1 = is_v ? p.vs1 : p.ks1;
@@ -337,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0)
       for (int j = max(0, i - NS); j < i; ++j) mbar_wait_bounded(&S.kv_full[j % NS], (j / NS) & 1);
     __syncwarp();
-  } else if (warp == kQkWarp) {
+  } else if (warp == SH::kQkWarp) {
     // ---------------- S^T = K Q^T -------------------------------------------------------
     if (lane == 0) {
       constexpr uint32_t kIdesc = tc::idesc_f16_f32(kTile, N, false);
@@ -362,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == kPvWarp) {
+  } else if (warp == SH::kPvWarp) {
     // ---------------- O^T += V^T P^T ----------------------------------------------------
     if (lane == 0) {
       constexpr uint32_t kIdesc = tc::idesc_f16_f32(kHead, N, true) | tc::kIdescAMnMajor;
@@ -372,15 +382,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0; w.next()) {
         const int n = w.count();
         for (int j = 0; j < n; ++j, ++i) {
-          const int st = i % NS, X = i & 1;
-          if (!failed) failed = !mbar_wait_bounded(&S.p_full[X], (i >> 1) & 1);
+          const int st = i % NS, X = i % G;
+          if (!failed) failed = !mbar_wait_bounded(&S.p_full[X], (i / G) & 1);
           if (!failed) {
             tc::fence_after_sync();
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
               tc::mma_f8(tbase + LK * N + X * N,
                          tc::sdesc_sw128(a_kv + st * 2 * kHalf + kHalf + ks * 32 * 128, kHalf, 1024),
-                         SH::p_desc(a_p + X * SH::kOperand + ks * 32 * N), kIdesc, j > 1 || ks != 0);
+                         SH::p_desc(a_p + X * SH::kOperand + ks * 32 * N), kIdesc, j >= G || ks != 0);
           }
           tc::commit(&S.pv_done[X]);
           tc::commit(&S.kv_empty[st]);
@@ -390,9 +400,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else {
     // ---------------- softmax groups ----------------------------------------------------
-    const int X = warp / kGroupWarps, gw = warp % kGroupWarps, gt = tid % (kGroupWarps * 32);
-    const uint32_t lane_off = (uint32_t)(gw * 32) << 16;
-    const uint32_t t_o = tbase + LK * N + X * N + lane_off;
+    const int X = warp / SH::kGroupWarps, part = warp % SH::kGroupWarps / 4, quad = warp % 4;
+    const int kt = quad * 32 + lane;  // the thread's key of a tile, and its dimension of O^T
+    const int r0 = part * RT;         // its first row
+    const int bar = 1 + X * SH::kParts + part;  // named barrier of the 128 threads of these rows
+    constexpr int kAll = 15;                    // and of all softmax threads
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const uint32_t t_o = tbase + LK * N + X * N + lane_off + r0;
     uint8_t* sp = smem + SH::kOffP + X * SH::kOperand;
     float* join = reinterpret_cast<float*>(smem + SH::kOffP);  // [R][kHead]
     bool failed = false;
@@ -401,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // per row (maximum in [2^7, 2^8)), two terms
     auto put_q = [&](const Span& s, int kh, int qb) {
       const int rows = s.qlen * p.group;
-      for (int e = tid; e < R * 8; e += kSoftWarps * 32) {
+      for (int e = tid; e < R * 8; e += kSoftThreads) {
         const int r = e >> 3, c = e & 7, t = r / p.group;
         uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if (r < rows) {
@@ -454,17 +468,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       // this one's end (the buffer's last reader ended with the segment before)
       w.next();
       if (w.left > 0) put_q(w.s, w.kh(), qb ^ 1);
-      if (gt < R) S.ref[X][gt] = kNone;
-      named_bar_sync(3, kSoftWarps * 32);  // factor, pos and ref are visible
+      if (kt < RT) S.ref[X][r0 + kt] = kNone;
+      named_bar_sync(kAll, kSoftThreads);  // factor, pos and ref are visible
 
-      float l[R];
+      float l[RT];
 #pragma unroll
-      for (int r = 0; r < R; ++r) l[r] = 0.f;
-      const int first = (i0 ^ X) & 1;  // the segment's first tile of this group
-      for (int j = first; j < n; j += 2) {
-        const int i = i0 + j, st = i % NS, k = i >> 1;  // k: the group's tiles so far
-        const int key0 = s.tile(off + j) * kTile, key = key0 + gt;
-        const uint32_t t_s = tbase + (i % LK) * N + lane_off;
+      for (int r = 0; r < RT; ++r) l[r] = 0.f;
+      const int first = (X + G - i0 % G) % G;  // the segment's first tile of this group
+      int k = (i0 + first) / G;                // the group's tiles so far
+      for (int j = first; j < n; j += G, ++k) {
+        const int i = i0 + j, st = i % NS;
+        const int key0 = s.tile(off + j) * kTile, key = key0 + kt;
+        const uint32_t t_s = tbase + (i % LK) * N + lane_off + r0;
         if (!failed) failed = !mbar_wait_bounded(&S.s_full[i % LK], (i / LK) & 1);
         tc::fence_after_sync();
         // all rows see the whole tile, or the mask is asked
@@ -473,116 +488,96 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool seen = open || (key < s.kv_end && (p.window == 0 || key > s.q0 - p.window || key < p.sinks));
         float ks = 0.f, lvs = 0.f, inv_vs = 0.f;
         if (seen) {
-          ks = S.scale[st][0][gt >> p.shift];
-          const float vs = fminf(fmaxf(S.scale[st][1][gt >> p.shift], kMinScale), kMaxScale);
+          ks = S.scale[st][0][kt >> p.shift];
+          const float vs = fminf(fmaxf(S.scale[st][1][kt >> p.shift], kMinScale), kMaxScale);
           lvs = __log2f(vs);
           inv_vs = __frcp_rn(vs);
         }
-        constexpr bool kKeep = R <= 32;  // the scores stay in registers, else they are read again
-        float x[kKeep ? R : CH];
-        auto scores = [&](int c, float* y) {  // y: scores of rows CH c ..
-          float hi[CH], lo[CH];
-          tc::ld_wait(t_s + CH * c, t_s + R + CH * c, hi, lo);
-          float f[CH];
-          row_values(f, S.factor[qb] + CH * c);
+        float x[RT], over = kMasked;
 #pragma unroll
-          for (int r = 0; r < CH; ++r) y[r] = fmaf(fmaf(lo[r], 1.f / kLo, hi[r]) * f[r], ks, lvs);
+        for (int c = 0; c < RT; c += CH) {
+          float hi[CH], lo[CH], f[CH], m[CH];
+          tc::ld_wait(t_s + c, t_s + R + c, hi, lo);
+          row_values(f, S.factor[qb] + r0 + c);
+          row_values(m, S.ref[X] + r0 + c);
+#pragma unroll
+          for (int r = 0; r < CH; ++r) x[c + r] = fmaf(fmaf(lo[r], 1.f / kLo, hi[r]) * f[r], ks, lvs);
           if (!open) {  // few tiles: a branch around all rows keeps the others' code short
 #pragma unroll
             for (int r = 0; r < CH; ++r) {
-              const int pos = S.pos[qb][CH * c + r];
-              if (!(seen && key <= pos && (p.window == 0 || key > pos - p.window || key < p.sinks))) y[r] = kMasked;
+              const int pos = S.pos[qb][r0 + c + r];
+              if (!(seen && key <= pos && (p.window == 0 || key > pos - p.window || key < p.sinks)))
+                x[c + r] = kMasked;
             }
           }
-        };
-        float over = kMasked;
 #pragma unroll
-        for (int c = 0; c < R / CH; ++c) {
-          float* y = kKeep ? x + CH * c : x;
-          scores(c, y);
-          float m[CH];
-          row_values(m, S.ref[X] + CH * c);
-#pragma unroll
-          for (int r = 0; r < CH; ++r) over = fmaxf(over, y[r] - m[r]);
+          for (int r = 0; r < CH; ++r) over = fmaxf(over, x[c + r] - m[r]);
         }
-        auto release = [&] {
-          tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&S.s_free[i % LK]);
-        };
-        if constexpr (kKeep) release();
-        const bool move = named_bar_or(1 + X, kGroupWarps * 32, over > kOff + kLazy);
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.s_free[i % LK]);
+        const bool move = named_bar_or(bar, 128, over > kOff + kLazy);
         // the group's previous product is done: P is free and O is stable
         if (k > 0 && !failed) failed = !mbar_wait_bounded(&S.pv_done[X], (k - 1) & 1);
         tc::fence_after_sync();
         if (move) {
 #pragma unroll
-          for (int c = 0; c < R / CH; ++c) {
-            float* y = kKeep ? x + CH * c : x;
-            if constexpr (!kKeep) scores(c, y);
-#pragma unroll
-            for (int r = 0; r < CH; ++r) {
-              const float m = warp_max(y[r]);
-              if (lane == (r & 31)) S.part_max[X][gw][CH * c + r] = m;
-            }
+          for (int r = 0; r < RT; ++r) {
+            const float m = warp_max(x[r]);
+            if (lane == r) S.part_max[X][quad][r0 + r] = m;
           }
-          named_bar_sync(1 + X, kGroupWarps * 32);
-          if (gt < R) {
-            const float top = fmaxf(fmaxf(S.part_max[X][0][gt], S.part_max[X][1][gt]),
-                                    fmaxf(S.part_max[X][2][gt], S.part_max[X][3][gt])) - kOff;
-            const float old = S.ref[X][gt], now = top > old + kLazy ? top : old;
-            S.ref[X][gt] = now;
-            S.alpha[X][gt] = ex2(old - now);
+          named_bar_sync(bar, 128);
+          if (kt < RT) {
+            const int a = r0 + kt;
+            const float top = fmaxf(fmaxf(S.part_max[X][0][a], S.part_max[X][1][a]),
+                                    fmaxf(S.part_max[X][2][a], S.part_max[X][3][a])) - kOff;
+            const float old = S.ref[X][a], now = top > old + kLazy ? top : old;
+            S.ref[X][a] = now;
+            S.alpha[X][a] = ex2(old - now);
           }
-          named_bar_sync(1 + X, kGroupWarps * 32);
+          named_bar_sync(bar, 128);
 #pragma unroll
-          for (int r = 0; r < R; ++r) l[r] *= S.alpha[X][r];
-          if (j > first) {
+          for (int c = 0; c < RT; c += 8) {
+            float a[8];
+            row_values(a, S.alpha[X] + r0 + c);
 #pragma unroll
-            for (int c = 0; c < R / CH; ++c) {
-              float hi[CH], lo[CH];
-              tc::ld_wait(t_o + CH * c, t_o + R + CH * c, hi, lo);
+            for (int r = 0; r < 8; ++r) l[c + r] *= a[r];
+            if (j > first) {
+              float hi[8], lo[8];
+              tc::ld_wait(t_o + c, t_o + R + c, hi, lo);
 #pragma unroll
-              for (int r = 0; r < CH; ++r) {
-                hi[r] *= S.alpha[X][CH * c + r];
-                lo[r] *= S.alpha[X][CH * c + r];
+              for (int r = 0; r < 8; ++r) {
+                hi[r] *= a[r];
+                lo[r] *= a[r];
               }
-              tc::st(t_o + CH * c, hi);
-              tc::st(t_o + R + CH * c, lo);
+              tc::st(t_o + c, hi);
+              tc::st(t_o + R + c, lo);
             }
-            tc::wait_st();
           }
+          tc::wait_st();
         }
+        uint32_t h[RT / 4], g[RT / 4];
 #pragma unroll
-        for (int c = 0; c < R / CH; ++c) {
-          float* y = kKeep ? x + CH * c : x;
-          if constexpr (!kKeep) scores(c, y);
-          float m[CH];
-          row_values(m, S.ref[X] + CH * c);
-          uint32_t h[CH / 4], g[CH / 4];
+        for (int c = 0; c < RT; c += 4) {
+          float m[4], hi[4], lo[4];
+          row_values(m, S.ref[X] + r0 + c);
 #pragma unroll
-          for (int r = 0; r < CH; r += 4) {
-            float hi[4], lo[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int a = CH * c + r + u;
-              const float pr = ex2(y[r + u] - m[r + u]);
-              l[a] = fmaf(pr, inv_vs, l[a]);
-              split4(pr, hi[u], lo[u]);
-            }
-            h[r / 4] = e4m3x2(hi[0], hi[1]) | (e4m3x2(hi[2], hi[3]) << 16);
-            g[r / 4] = e4m3x2(lo[0] * kLo, lo[1] * kLo) | (e4m3x2(lo[2] * kLo, lo[3] * kLo) << 16);
+          for (int u = 0; u < 4; ++u) {
+            const float pr = ex2(x[c + u] - m[u]);
+            l[c + u] = fmaf(pr, inv_vs, l[c + u]);
+            split4(pr, hi[u], lo[u]);
           }
-          if constexpr (R == 8) {
-            *reinterpret_cast<uint4*>(sp + SH::p_at(gt, 0)) = make_uint4(h[0], h[1], g[0], g[1]);
-          } else {
-            *reinterpret_cast<uint4*>(sp + SH::p_at(gt, c)) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(sp + SH::p_at(gt, R / 16 + c)) = make_uint4(g[0], g[1], g[2], g[3]);
-          }
+          h[c / 4] = e4m3x2(hi[0], hi[1]) | (e4m3x2(hi[2], hi[3]) << 16);
+          g[c / 4] = e4m3x2(lo[0] * kLo, lo[1] * kLo) | (e4m3x2(lo[2] * kLo, lo[3] * kLo) << 16);
         }
-        if constexpr (!kKeep) release();
-        if (!seen) {
-          uint4* v = reinterpret_cast<uint4*>(smem + st * 2 * kHalf + kHalf + gt * kHead);
+        if constexpr (R == 8) {
+          *reinterpret_cast<uint4*>(sp + SH::p_at(kt, 0)) = make_uint4(h[0], h[1], g[0], g[1]);
+        } else {
+          *reinterpret_cast<uint4*>(sp + SH::p_at(kt, part)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(sp + SH::p_at(kt, R / 16 + part)) = make_uint4(g[0], g[1], g[2], g[3]);
+        }
+        if (!seen && part == 0) {
+          uint4* v = reinterpret_cast<uint4*>(smem + st * 2 * kHalf + kHalf + kt * kHead);
 #pragma unroll
           for (int c = 0; c < 8; ++c) v[c] = make_uint4(0, 0, 0, 0);
         }
@@ -593,52 +588,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 
       // ---- the segment's end: join the groups, store or leave a partial ------------------
-      const int own = (n - first + 1) / 2;  // tiles of this group
-      const int klast = (i0 + first + 2 * (own - 1)) >> 1;
-      if (own > 0 && !failed) failed = !mbar_wait_bounded(&S.pv_done[X], klast & 1);
+      const bool own = first < n;
+      if (own && !failed) failed = !mbar_wait_bounded(&S.pv_done[X], (k - 1) & 1);
       tc::fence_after_sync();
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
+      for (int r = 0; r < RT; ++r) {
         float v = l[r];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == (r & 31)) S.fin_l[X][gw][r] = v;
+        if (lane == r) S.fin_l[X][quad][r0 + r] = v;
       }
-      if (gt < R) S.fin_m[X][gt] = S.ref[X][gt];  // kNone where the group had no tile
-      named_bar_sync(3, kSoftWarps * 32);
+      if (kt < RT) S.fin_m[X][r0 + kt] = S.ref[X][r0 + kt];  // kNone where the group had no tile
+      named_bar_sync(kAll, kSoftThreads);
       auto weight = [&](int g, int r) {  // of group g in row r's sum
-        return ex2(S.fin_m[g][r] - fmaxf(S.fin_m[g][r], S.fin_m[g ^ 1][r]));
+        return G == 1 ? 1.f : ex2(S.fin_m[g][r] - fmaxf(S.fin_m[0][r], S.fin_m[1][r]));
       };
-      auto output = [&](int c, float (&o)[CH]) {  // this group's O^T of rows CH c .., dimension gt
-        float lo[CH];
-        tc::ld_wait(t_o + CH * c, t_o + R + CH * c, o, lo);
+      const bool other = G == 2 && n > (1 + G - i0 % G) % G;  // group 1 had a tile
 #pragma unroll
-        for (int r = 0; r < CH; ++r) o[r] = fmaf(lo[r], 1.f / kLo, o[r]) * weight(X, CH * c + r);
-      };
-      if (X == 1 && own > 0) {
+      for (int g = G - 1; g >= 0; --g) {
+        if (X == g && own) {
 #pragma unroll
-        for (int c = 0; c < R / CH; ++c) {
-          float o[CH];
-          output(c, o);
+          for (int c = 0; c < RT; c += 8) {
+            float hi[8], lo[8];
+            tc::ld_wait(t_o + c, t_o + R + c, hi, lo);
 #pragma unroll
-          for (int r = 0; r < CH; ++r) join[(CH * c + r) * kHead + gt] = o[r];
-        }
-      }
-      const bool other = n - ((i0 ^ 1) & 1) > 0;  // group 1 had a tile
-      named_bar_sync(3, kSoftWarps * 32);
-      if (X == 0 && (own > 0 || other)) {
-#pragma unroll
-        for (int c = 0; c < R / CH; ++c) {
-          float o[CH];
-          if (own > 0) output(c, o);
-#pragma unroll
-          for (int r = 0; r < CH; ++r) {
-            const int a = (CH * c + r) * kHead + gt;
-            if (own > 0) join[a] = other ? join[a] + o[r] : o[r];
+            for (int r = 0; r < 8; ++r) {
+              float* at = join + (r0 + c + r) * kHead + kt;
+              const float o = fmaf(lo[r], 1.f / kLo, hi[r]) * weight(g, r0 + c + r);
+              *at = g == 0 && other ? *at + o : o;
+            }
           }
         }
+        named_bar_sync(kAll, kSoftThreads);
       }
-      named_bar_sync(3, kSoftWarps * 32);
       auto store = [&](int a, int c, float4 o, float sum) {  // row a, dimensions 4 c ..
         const float f = sum > 0.f ? __fdividef(1.f, sum) : 0.f;
         const int t = a / p.group;
@@ -648,41 +630,40 @@ __global__ void __launch_bounds__(kThreads, 1)
             make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
       };
       const bool whole = n == s.tiles;
-      constexpr int kPart = kMaxRows * (kHead + 2);
-      float* part = p.partials + (int64_t)(2 * blockIdx.x + (item >= begin ? 1 : 0)) * kPart;
-      for (int e = tid; e < rows * (kHead / 4); e += kSoftWarps * 32) {
+      float* part_o = p.partials + (int64_t)(2 * blockIdx.x + (item >= begin ? 1 : 0)) * kPart;
+      for (int e = tid; e < rows * (kHead / 4); e += kSoftThreads) {
         const int a = e / (kHead / 4), c = e % (kHead / 4);
         const float4 o = *reinterpret_cast<const float4*>(join + a * kHead + 4 * c);
         float sum = 0.f;
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int g = 0; g < G; ++g)
           sum += weight(g, a) * (S.fin_l[g][0][a] + S.fin_l[g][1][a] + S.fin_l[g][2][a] + S.fin_l[g][3][a]);
         if (whole) {
           store(a, c, o, sum);
         } else {
-          *reinterpret_cast<float4*>(part + a * kHead + 4 * c) = o;
+          *reinterpret_cast<float4*>(part_o + a * kHead + 4 * c) = o;
           if (c == 0)
-            *reinterpret_cast<float2*>(part + kMaxRows * kHead + 2 * a) =
-                make_float2(fmaxf(S.fin_m[0][a], S.fin_m[1][a]), sum);
+            *reinterpret_cast<float2*>(part_o + kMaxRows * kHead + 2 * a) =
+                make_float2(G == 1 ? S.fin_m[0][a] : fmaxf(S.fin_m[0][a], S.fin_m[1][a]), sum);
         }
       }
       if (!whole) {
-        __threadfence();
-        named_bar_sync(3, kSoftWarps * 32);
+        named_bar_sync(kAll, kSoftThreads);
         const int c_lo = share_owner(item, total, shares), c_hi = share_owner(item + s.tiles - 1, total, shares);
         if (tid == 0) {
           int* counter = p.counters + (int64_t)seq * p.hkv + kh;
+          __threadfence();  // the other threads' partials, which the barrier has ordered before this
           S.last = atomicAdd(counter, 1) == c_hi - c_lo;
           if (S.last) *counter = 0;
-        }
-        named_bar_sync(3, kSoftWarps * 32);
-        if (S.last) {
           __threadfence();
+        }
+        named_bar_sync(kAll, kSoftThreads);
+        if (S.last) {
           // the shares of the item in order, kJoin loads of each kind in flight
-          constexpr int kJoin = 8;
+          constexpr int kJoin = R <= 16 ? 8 : 4;
           // later shares begin inside the item: it is their first
           const int at0 = item >= share_begin(c_lo, total, shares) ? 1 : 0;
-          for (int e = tid; e < rows * (kHead / 4); e += kSoftWarps * 32) {
+          for (int e = tid; e < rows * (kHead / 4); e += kSoftThreads) {
             const int a = e / (kHead / 4), c = e % (kHead / 4);
             float top = kNone, sum = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -719,24 +700,28 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      named_bar_sync(3, kSoftWarps * 32);  // P and the exchange buffers are free
+      named_bar_sync(kAll, kSoftThreads);  // P and the exchange buffers are free
       i0 += n;
     }
   }
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == kQkWarp) tc::tmem_dealloc(tbase, SH::kTmem);
+  if (warp == SH::kQkWarp) tc::tmem_dealloc(tbase, SH::kTmem);
 }
 
 template <int R>
 cudaError_t launch(const CUtensorMap& km, const CUtensorMap& vm, const BlockAttnParams& p, int ctas, cudaStream_t st) {
   const int smem = Shape<R>::kBytes + 1024;
-  const cudaError_t e =
-      cudaFuncSetAttribute(block_decode_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
+  static PerDevice sized;
+  if (!sized.done()) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(block_decode_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    sized.set();
+  }
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(ctas, 1, 1);
-  lc.blockDim = dim3(kThreads, 1, 1);
+  lc.blockDim = dim3(Shape<R>::kThreads, 1, 1);
   lc.dynamicSmemBytes = smem;
   lc.stream = st;
   cudaLaunchAttribute attr[1];

@@ -64,5 +64,5 @@ def verify(logits, tokens, cu_rows, uniforms, noise, temperature=None, draft_pro
         temperature.data_ptr() if temperature is not None else None,
         draft_probs.data_ptr() if draft_probs is not None else None,
         draft_probs.stride(0) if draft_probs is not None else 0, out_tokens.data_ptr(), num_accepted.data_ptr(), seqs,
-        rows, vocab, torch.cuda.current_stream(logits.device).cuda_stream), "b200kv_spec_verify")
+        rows, vocab, torch._C._cuda_getCurrentRawStream(logits.device.index)), "b200kv_spec_verify")
     return out_tokens, num_accepted
