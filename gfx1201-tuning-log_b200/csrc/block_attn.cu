@@ -1,12 +1,9 @@
-// Causal attention over a block-scaled fp8 paged cache (sm_100a).
-//
-// The plain kernel: one CTA per (query token, kv head), one thread per key for
-// the scores and one per dimension for the output, fp32 throughout, an online
-// softmax over chunks of 128 keys.
+// Causal attention over a block-scaled fp8 paged cache: arguments, workspace and
+// the split of a batch between the few-query kernel (block_decode.cu) and the
+// many-query one (block_prefill.cu), each of which leaves the other's sequences.
 
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
-#include <cuda_fp8.h>
 #include <stdint.h>
 
 #include "b200kv.h"
@@ -21,107 +18,31 @@ int block_cache_check(const b200kv_block_cache* c);
 namespace {
 
 constexpr int kHead = 128;
-
-__device__ __forceinline__ float e4m3(uint8_t b) {
-  const __half_raw h = __nv_cvt_fp8_to_halfraw(b, __NV_E4M3);
-  return __half2float(*reinterpret_cast<const __half*>(&h));
-}
-
-__global__ void __launch_bounds__(kHead) block_attn_plain_kernel(const BlockAttnParams p) {
-  __shared__ float s_q[kMaxGroup][kHead], s_p[kMaxGroup][kHead], s_red[kHead / 32][kMaxGroup];
-  __shared__ float s_vs[kHead];
-  __shared__ int64_t s_v[kHead];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x, kh = blockIdx.y, G = p.group;
-  griddep_wait();
-  int seq = 0;
-  while (seq + 1 < p.num_seqs && p.cu[seq + 1] <= row) ++seq;
-  if (row < p.cu[seq] || row >= p.cu[seq + 1]) return;
-  if ((p.cu[seq + 1] - p.cu[seq]) * G <= kMaxRows) return;  // the few-query kernel's
-  const int pos = p.lens[seq] - (p.cu[seq + 1] - row);
-  for (int g = 0; g < G; ++g)
-    s_q[g][tid] = __bfloat162float(p.q[(int64_t)row * p.q_st + (int64_t)(kh * G + g) * p.q_sh + tid]);
-  __syncthreads();
-  float m[kMaxGroup], l[kMaxGroup], o[kMaxGroup];
-#pragma unroll
-  for (int g = 0; g < kMaxGroup; ++g) { m[g] = -INFINITY; l[g] = 0.f; o[g] = 0.f; }
-  for (int base = 0; base <= pos; base += kHead) {
-    const int j = base + tid;
-    const int page = j >> p.shift;
-    const bool sees = j <= pos && page < p.max_blocks && (p.window == 0 || j > pos - p.window || j < p.sinks);
-    if (!__syncthreads_or(sees)) continue;
-    float sc[kMaxGroup];
-#pragma unroll
-    for (int g = 0; g < kMaxGroup; ++g) sc[g] = -INFINITY;
-    s_vs[tid] = 0.f;
-    s_v[tid] = -1;
-    if (sees) {
-      const int blk = p.bt[(int64_t)seq * p.bt_stride + page], slot = j & ((1 << p.shift) - 1);
-      const bool ok = blk >= 0 && blk < p.num_blocks;
-#pragma unroll
-      for (int g = 0; g < kMaxGroup; ++g) sc[g] = 0.f;
-      if (ok) {
-        const uint8_t* kp = p.kc + (int64_t)blk * p.sk0 + (int64_t)slot * p.sk1 + (int64_t)kh * p.sk2;
-        for (int d = 0; d < kHead; ++d) {
-          const float kv = e4m3(kp[d]);
-#pragma unroll
-          for (int g = 0; g < kMaxGroup; ++g)
-            if (g < G) sc[g] += s_q[g][d] * kv;
-        }
-        const float f = p.sm_scale * p.ks[(int64_t)blk * p.ks0 + kh * p.ks1];
-#pragma unroll
-        for (int g = 0; g < kMaxGroup; ++g) sc[g] *= f;
-        s_vs[tid] = p.vs[(int64_t)blk * p.vs0 + kh * p.vs1];
-        s_v[tid] = (int64_t)blk * p.sv0 + (int64_t)slot * p.sv1 + (int64_t)kh * p.sv2;
-      }
-    }
-#pragma unroll
-    for (int g = 0; g < kMaxGroup; ++g) {
-      if (g >= G) break;
-      float v = sc[g];
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
-      if (lane == 0) s_red[warp][g] = v;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int g = 0; g < kMaxGroup; ++g) {
-      if (g >= G) break;
-      float v = m[g];
-#pragma unroll
-      for (int w = 0; w < kHead / 32; ++w) v = fmaxf(v, s_red[w][g]);
-      const float a = m[g] == v ? 1.f : __expf(m[g] - v);
-      m[g] = v;
-      l[g] *= a;
-      o[g] *= a;
-      s_p[g][tid] = sees ? __expf(sc[g] - v) : 0.f;
-    }
-    __syncthreads();
-    for (int t = 0; t < kHead; ++t) {
-      const float x = s_v[t] >= 0 ? e4m3(p.vc[s_v[t] + tid]) * s_vs[t] : 0.f;
-#pragma unroll
-      for (int g = 0; g < kMaxGroup; ++g)
-        if (g < G) {
-          l[g] += s_p[g][t];
-          o[g] += s_p[g][t] * x;
-        }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int g = 0; g < kMaxGroup; ++g)
-    if (g < G)
-      p.out[(int64_t)row * p.o_st + (int64_t)(kh * G + g) * p.o_sh + tid] =
-          __float2bfloat16_rn(l[g] > 0.f ? o[g] / l[g] : 0.f);
-}
+constexpr size_t kCounterBytes = 1024;                    // kMaxCtas counters
+constexpr size_t kRecordBytes = kMaxCtas * 8 * sizeof(int);
+static_assert(kMaxCtas * sizeof(int) <= kCounterBytes && kRecordBytes % 256 == 0, "workspace layout");
 
 }  // namespace
 
-// counters, then the partials
+int block_attn_shares(BlockAttnParams* p) {
+  const int sms = num_sms_current_device() < kMaxCtas ? num_sms_current_device() : kMaxCtas;
+  int ctas = 0;
+  for (int heads = 1; heads <= p->hkv; ++heads) {
+    if (p->hkv % heads) continue;
+    const int slots = p->hkv / heads, n = sms / slots * slots;
+    if (n > ctas + ctas / 16) {
+      ctas = n;
+      p->heads = heads;
+      p->slots = slots;
+    }
+  }
+  return ctas;
+}
+
+// counters, records, partials
 size_t block_attn_workspace_bytes(int num_seqs, int num_kv_heads) {
   if (num_seqs <= 0 || num_kv_heads <= 0) return 0;
-  return align_up((size_t)num_seqs * num_kv_heads * sizeof(int), 256) +
-         (size_t)2 * kMaxCtas * kMaxRows * (kHead + 2) * sizeof(float);
+  return kCounterBytes + kRecordBytes + (size_t)2 * kMaxCtas * kPartialFloats * sizeof(float);
 }
 
 int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args* a, void* stream) {
@@ -165,9 +86,10 @@ int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args*
   p.window = a->window;
   p.sinks = a->sinks;
   p.hkv = c->num_kv_heads;
-  p.counters = static_cast<int*>(a->workspace);
-  p.partials = reinterpret_cast<float*>(static_cast<char*>(a->workspace) +
-                                        align_up((size_t)c->num_seqs * c->num_kv_heads * sizeof(int), 256));
+  char* ws = static_cast<char*>(a->workspace);
+  p.counters = reinterpret_cast<int*>(ws);
+  p.records = reinterpret_cast<int*>(ws + kCounterBytes);
+  p.partials = reinterpret_cast<float*>(ws + kCounterBytes + kRecordBytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   CUtensorMap km, vm;
   if (!encode_paged_kv(&km, c->k, kHead, (uint32_t)c->num_kv_heads, (uint32_t)c->block_size, (uint64_t)c->num_blocks,
@@ -176,11 +98,10 @@ int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args*
                        (uint64_t)c->sv2, (uint64_t)c->sv1, (uint64_t)c->sv0))
     return B200KV_ERR_UNSUPPORTED;
   const int64_t rows = (int64_t)a->max_qlen * p.group;
-  if (block_decode_launch(km, vm, p, rows < kMaxRows ? (int)rows : kMaxRows, st) != cudaSuccess)
-    return B200KV_ERR_LAUNCH;
-  if (rows <= kMaxRows) return B200KV_OK;
-  block_attn_plain_kernel<<<dim3(a->num_tokens, c->num_kv_heads), kHead, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? B200KV_OK : B200KV_ERR_LAUNCH;
+  cudaError_t e = cudaSuccess;
+  if (rows > kMaxRows) e = block_prefill_launch(km, vm, p, st);
+  if (e == cudaSuccess) e = block_decode_launch(km, vm, p, rows < kMaxRows ? (int)rows : kMaxRows, st);
+  return e == cudaSuccess ? B200KV_OK : B200KV_ERR_LAUNCH;
 }
 
 }  // namespace b200kv

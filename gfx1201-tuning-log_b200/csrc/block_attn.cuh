@@ -12,7 +12,9 @@ namespace b200kv {
 
 constexpr int kMaxGroup = 16;  // query heads per kv head
 constexpr int kMaxRows = 64;   // (query token, head) rows of a kv head that the few-query kernel takes
-constexpr int kMaxCtas = 160;  // shares of a batch it is cut into, at most
+constexpr int kMaxCtas = 160;  // of a launch
+constexpr int kPairRows = 256;  // rows of a kv head that a CTA of the many-query kernel holds
+constexpr int kPartialFloats = kPairRows * (128 + 2);  // o, then (m, l) of each row
 
 // Whether something was done once on the current device (a kernel's attribute set).
 class PerDevice {
@@ -50,13 +52,49 @@ struct BlockAttnParams {
   int64_t sk0, sk1, sk2, sv0, sv1, sv2, ks0, ks1, vs0, vs1;
   float sm_scale;
   int num_seqs, hkv, group, shift, num_blocks, max_blocks, window, sinks;
-  int heads, slots;  // of the few-query kernel: kv heads a CTA walks, CTAs that share a range
-  float* partials;  // [2 kMaxCtas][kMaxRows x (128 + m + l)]
-  int* counters;    // [num_seqs][hkv], zero between calls
+  // The batch's key tiles, ordered by (sequence, kv head, queries, tile), are cut into
+  // equal shares; `slots` CTAs walk a share at once, each for `heads` of the kv heads.
+  int heads, slots;
+  float* partials;  // two a CTA: what a share leaves of an item that it cuts
+  int* counters;    // [kMaxCtas], zero between calls: arrivals at the item cut at a CTA's end
+  int* records;     // [kMaxCtas][8]: the many-query kernel's cut items, for the join after it
 };
+
+// The 128-key tiles that the queries at positions first .. see, of keys [0, kv_end):
+// tiles 0 .. sinks - 1, then low ..
+struct KeyTiles {
+  int sinks, low, count;
+  __device__ __forceinline__ int tile(int j) const { return j < sinks ? j : low + j - sinks; }
+};
+__device__ __forceinline__ KeyTiles key_tiles(const BlockAttnParams& p, int first, int kv_end) {
+  KeyTiles t = {0, 0, 0};
+  if (kv_end <= 0) return t;
+  const int high = (kv_end - 1) / 128 + 1;
+  if (p.window > 0) {
+    t.low = min(max(0, first - p.window + 1) / 128, high);
+    t.sinks = p.sinks > 0 ? min((min(p.sinks, kv_end) - 1) / 128 + 1, t.low) : 0;
+  }
+  t.count = t.sinks + high - t.low;
+  return t;
+}
+
+// Share i of `shares` begins at tile i total / shares; the owner of a tile is the
+// last share that does not begin past it.
+__device__ __forceinline__ int64_t share_begin(int64_t share, int64_t total, int64_t shares) {
+  return share * total / shares;
+}
+__device__ __forceinline__ int share_owner(int64_t tile, int64_t total, int64_t shares) {
+  return (int)(((tile + 1) * shares - 1) / total);
+}
+
+// Sets p.heads and p.slots and returns the CTAs to launch: the fewest kv heads a CTA
+// that keep the most SMs busy (8 heads: one each on 18 x 8 = 144 of 148 SMs).
+int block_attn_shares(BlockAttnParams* p);
 
 // sequences with at most kMaxRows rows per kv head; `rows` bounds them in this batch
 cudaError_t block_decode_launch(const CUtensorMap& km, const CUtensorMap& vm, BlockAttnParams p, int rows,
                                 cudaStream_t st);
+// the others
+cudaError_t block_prefill_launch(const CUtensorMap& km, const CUtensorMap& vm, BlockAttnParams p, cudaStream_t st);
 
 }  // namespace b200kv

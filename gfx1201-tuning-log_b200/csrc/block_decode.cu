@@ -55,7 +55,7 @@ namespace {
 constexpr int kHead = 128;
 constexpr int kTile = 128;                  // keys per tile
 constexpr int kHalf = kTile * kHead;        // K (or V) bytes of a tile
-constexpr int kPart = kMaxRows * (kHead + 2);  // floats of a partial: o, then (m, l) of each row
+static_assert(kMaxRows * (kHead + 2) <= kPartialFloats, "a partial holds the rows");
 constexpr int kMaxPages = 8;                // pages per tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 4.f;                // the reference moves when a maximum exceeds it by 2^4
@@ -148,8 +148,7 @@ __device__ __forceinline__ void async_arrive(uint64_t* bar) {
 // The tiles of one sequence that any of its queries sees.
 struct Span {
   int qlen, total, kv_end, q0, row0;
-  int sink_tiles, low_tile, tiles;  // tiles 0 .. sink_tiles - 1, then low_tile ..
-  __device__ __forceinline__ int tile(int j) const { return j < sink_tiles ? j : low_tile + j - sink_tiles; }
+  KeyTiles keys;
 };
 __device__ __forceinline__ Span span_of(const BlockAttnParams& p, int seq, int max_rows) {
   Span s;
@@ -158,15 +157,8 @@ __device__ __forceinline__ Span span_of(const BlockAttnParams& p, int seq, int m
   s.total = p.lens[seq];
   s.q0 = s.total - s.qlen;
   s.kv_end = min(s.total, p.max_blocks << p.shift);
-  s.tiles = s.sink_tiles = s.low_tile = 0;
-  if (s.qlen <= 0 || s.qlen > max_rows || s.qlen * p.group > max_rows || s.kv_end <= 0) return s;
-  const int high = (s.kv_end + kTile - 1) / kTile;
-  if (p.window > 0) {
-    s.low_tile = min(max(0, s.q0 - p.window + 1) / kTile, high);
-    s.sink_tiles = min(min(p.sinks, s.kv_end) + kTile - 1, s.kv_end + kTile - 1) / kTile;
-    s.sink_tiles = min(s.sink_tiles, s.low_tile);
-  }
-  s.tiles = s.sink_tiles + high - s.low_tile;
+  s.keys.count = 0;
+  if (s.qlen > 0 && s.qlen <= max_rows && s.qlen * p.group <= max_rows) s.keys = key_tiles(p, s.q0, s.kv_end);
   return s;
 }
 
@@ -182,32 +174,25 @@ struct Walk {
       : p(p_), max_rows(max_rows_), seq(seq_), left(count) {
     s = span_of(p, seq, max_rows);
     const int rel = (int)(begin - (int64_t)prefix * p.heads);
-    sub = rel / s.tiles;
-    off = rel - sub * s.tiles;
+    sub = rel / s.keys.count;
+    off = rel - sub * s.keys.count;
     item = begin - off;
   }
-  __device__ __forceinline__ int count() const { return min(s.tiles - off, left); }
+  __device__ __forceinline__ int count() const { return min(s.keys.count - off, left); }
   __device__ __forceinline__ int kh() const { return blockIdx.x % p.slots * p.heads + sub; }
   __device__ __forceinline__ void next() {
     left -= count();
     if (left <= 0) return;
-    item += s.tiles;
+    item += s.keys.count;
     off = 0;
     if (++sub == p.heads) {
       sub = 0;
       do {
         s = span_of(p, ++seq, max_rows);
-      } while (s.tiles == 0 && seq + 1 < p.num_seqs);
+      } while (s.keys.count == 0 && seq + 1 < p.num_seqs);
     }
   }
 };
-
-__device__ __forceinline__ int64_t share_begin(int64_t share, int64_t total, int64_t shares) {
-  return share * total / shares;
-}
-__device__ __forceinline__ int share_owner(int64_t tile, int64_t total, int64_t shares) {
-  return (int)(((tile + 1) * shares - 1) / total);
-}
 
 template <int R>
 __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
@@ -246,7 +231,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
   const int per = (p.num_seqs + kThreads - 1) / kThreads;
   const int s_lo = min(p.num_seqs, tid * per), s_hi = min(p.num_seqs, s_lo + per);
   int mine = 0;
-  for (int s = s_lo; s < s_hi; ++s) mine += span_of(p, s, R).tiles;
+  for (int s = s_lo; s < s_hi; ++s) mine += span_of(p, s, R).keys.count;
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -273,7 +258,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
     int at = before + incl - mine;  // tiles of the sequences before this thread's
     if (begin >= (int64_t)at * p.heads && begin < (int64_t)(at + mine) * p.heads)
       for (int s = s_lo; s < s_hi; ++s) {
-        const int n = span_of(p, s, R).tiles;
+        const int n = span_of(p, s, R).keys.count;
         if (begin < (int64_t)(at + n) * p.heads) {
           S.first_seq = s;
           S.first_prefix = at;
@@ -289,7 +274,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
     // queries of sequences without a key: zeros
     for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
       const Span sp = span_of(p, s, R);
-      if (sp.tiles == 0 && sp.qlen > 0 && sp.qlen <= R && sp.qlen * p.group <= R)
+      if (sp.keys.count == 0 && sp.qlen > 0 && sp.qlen <= R && sp.qlen * p.group <= R)
         for (int i = lane; i < sp.qlen * p.hkv * p.group * kHead; i += 32) {
           const int t = i / (p.hkv * p.group * kHead), h = i / kHead % (p.hkv * p.group);
           p.out[(int64_t)(sp.row0 + t) * p.o_st + (int64_t)h * p.o_sh + i % kHead] = __float2bfloat16_rn(0.f);
@@ -314,7 +299,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
       auto entry = [&](int j0) {  // block of this lane's page of tiles j0 ..
         const int j = j0 + lane / ppt;
         if (j >= n) return -1;
-        const int page = w.s.tile(w.off + j) * ppt + lane % ppt;
+        const int page = w.s.keys.tile(w.off + j) * ppt + lane % ppt;
         return page << p.shift < w.s.kv_end ? __ldg(row + page) : -1;
       };
       int cur = entry(0), nxt = entry(tpw);
@@ -330,7 +315,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
           ok = false;
           break;
         }
-        const int keys = min(kTile, w.s.kv_end - w.s.tile(w.off + j) * kTile);
+        const int keys = min(kTile, w.s.kv_end - w.s.keys.tile(w.off + j) * kTile);
         const int pages = (keys + bs - 1) >> p.shift;
         if (lane == 0) mbar_arrive_expect_tx(&S.kv_full[st], (uint32_t)(pages * bs * kHead));
         __syncwarp();
@@ -460,7 +445,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
     Walk w(p, R, S.first_seq, S.first_prefix, begin, count);
     put_q(w.s, w.kh(), 0);
     for (; w.left > 0; ++seg) {
-      const int n = w.count(), qb = seg & 1, kh = w.kh(), seq = w.seq;
+      const int n = w.count(), qb = seg & 1, kh = w.kh();
       const Span s = w.s;
       const int64_t item = w.item;
       const int off = w.off, rows = s.qlen * p.group;
@@ -478,7 +463,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
       int k = (i0 + first) / G;                // the group's tiles so far
       for (int j = first; j < n; j += G, ++k) {
         const int i = i0 + j, st = i % NS;
-        const int key0 = s.tile(off + j) * kTile, key = key0 + kt;
+        const int key0 = s.keys.tile(off + j) * kTile, key = key0 + kt;
         const uint32_t t_s = tbase + (i % LK) * N + lane_off + r0;
         if (!failed) failed = !mbar_wait_bounded(&S.s_full[i % LK], (i / LK) & 1);
         tc::fence_after_sync();
@@ -629,8 +614,8 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
                                   (int64_t)(kh * p.group + a - t * p.group) * p.o_sh + 4 * c) =
             make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
       };
-      const bool whole = n == s.tiles;
-      float* part_o = p.partials + (int64_t)(2 * blockIdx.x + (item >= begin ? 1 : 0)) * kPart;
+      const bool whole = n == s.keys.count;
+      float* part_o = p.partials + (int64_t)(2 * blockIdx.x + (item >= begin ? 1 : 0)) * kPartialFloats;
       for (int e = tid; e < rows * (kHead / 4); e += kSoftThreads) {
         const int a = e / (kHead / 4), c = e % (kHead / 4);
         const float4 o = *reinterpret_cast<const float4*>(join + a * kHead + 4 * c);
@@ -649,9 +634,9 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
       }
       if (!whole) {
         named_bar_sync(kAll, kSoftThreads);
-        const int c_lo = share_owner(item, total, shares), c_hi = share_owner(item + s.tiles - 1, total, shares);
+        const int c_lo = share_owner(item, total, shares), c_hi = share_owner(item + s.keys.count - 1, total, shares);
         if (tid == 0) {
-          int* counter = p.counters + (int64_t)seq * p.hkv + kh;
+          int* counter = p.counters + c_lo * p.slots + slot;  // one item at most is cut at a share's end
           __threadfence();  // the other threads' partials, which the barrier has ordered before this
           S.last = atomicAdd(counter, 1) == c_hi - c_lo;
           if (S.last) *counter = 0;
@@ -677,7 +662,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
                 v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (c0 + u <= c_hi) {
                   const int64_t cta = (int64_t)(c0 + u) * p.slots + slot;
-                  const float* q = p.partials + (2 * cta + (c0 + u == c_lo ? at0 : 0)) * kPart;
+                  const float* q = p.partials + (2 * cta + (c0 + u == c_lo ? at0 : 0)) * kPartialFloats;
                   ml[u] = __ldcg(reinterpret_cast<const float2*>(q + kMaxRows * kHead + 2 * a));
                   v[u] = __ldcg(reinterpret_cast<const float4*>(q + a * kHead + 4 * c));
                 }
@@ -736,19 +721,7 @@ cudaError_t launch(const CUtensorMap& km, const CUtensorMap& vm, const BlockAttn
 
 cudaError_t block_decode_launch(const CUtensorMap& km, const CUtensorMap& vm, BlockAttnParams p, int rows,
                                 cudaStream_t st) {
-  // kv heads walked by one CTA, one after the other: the fewest that keep the most
-  // SMs busy (8 heads: one each on 18 x 8 = 144 of 148 SMs)
-  const int sms = num_sms_current_device() < kMaxCtas ? num_sms_current_device() : kMaxCtas;
-  int ctas = 0;
-  for (int heads = 1; heads <= p.hkv; ++heads) {
-    if (p.hkv % heads) continue;
-    const int slots = p.hkv / heads, n = sms / slots * slots;
-    if (n > ctas + ctas / 16) {
-      ctas = n;
-      p.heads = heads;
-      p.slots = slots;
-    }
-  }
+  const int ctas = block_attn_shares(&p);
   if (rows <= 8) return launch<8>(km, vm, p, ctas, st);
   if (rows <= 16) return launch<16>(km, vm, p, ctas, st);
   if (rows <= 32) return launch<32>(km, vm, p, ctas, st);
