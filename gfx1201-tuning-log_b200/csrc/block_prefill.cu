@@ -54,6 +54,7 @@ constexpr float kLazy = 4.f;
 constexpr float kFar = 10.f;             // log2 of how far apart blocks' scales may be for f16 sums
 constexpr float kMinScale = 8.2718061e-25f, kMaxScale = 1.2089258e24f;  // 2^-80, 2^80
 constexpr float kNone = -1e30f;          // the reference of a row that has seen no key
+constexpr float kTiny = 1e-37f;          // a factor of zero becomes it, so that a hidden key stays -inf
 
 // shared memory
 constexpr int kOffQ = 0;                          // [query tile][hi, lo]
@@ -491,14 +492,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       // skips would else let these warps run ahead of its barriers)
       if (seg > 0 && !failed) failed = !mbar_wait_bounded(&S.q_free[X], (seg - 1) & 1);
       {
-        // Q: a power-of-two prescale (maximum in [2^7, 2^8)) with the sign of sm_scale, two terms
+        // Q: a power-of-two prescale (maximum in [2^7, 2^8)) with the sign of sm_scale, two
+        // terms; the row is read twice, the second time from L1
         const uint4* src = reinterpret_cast<const uint4*>(p.q + q_row * p.q_st + (int64_t)head * p.q_sh);
-        uint4 raw[16];
+        const uint4 zero = make_uint4(0, 0, 0, 0);
         float mx = 0.f;
-#pragma unroll
+#pragma unroll 4
         for (int c = 0; c < 16; ++c) {
-          raw[c] = valid ? src[c] : make_uint4(0, 0, 0, 0);
-          const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+          const uint4 w4 = valid ? __ldg(src + c) : zero;
+          const uint32_t u[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(u[k] << 16)), fabsf(__uint_as_float(u[k] & 0xFFFF0000u))));
@@ -509,12 +511,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         float up = __uint_as_float((uint32_t)(sh + 127) << 23);
         if (p.sm_scale < 0.f) up = -up;
         uint8_t* q = smem + kOffQ + 2 * X * kBytes8;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 8; ++c) {
           float v[16];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t u[4] = {raw[2 * c + h].x, raw[2 * c + h].y, raw[2 * c + h].z, raw[2 * c + h].w};
+            const uint4 w4 = valid ? __ldg(src + 2 * c + h) : zero;
+            const uint32_t u[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               v[8 * h + 2 * k] = __uint_as_float(u[k] << 16) * up;
@@ -546,21 +549,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after_sync();
         const bool open = key0 + kTile - 1 <= r.first(X) && key0 + kTile <= r.kv_end &&
                           (p.window == 0 || key0 > r.last(X) - p.window || key0 + kTile <= p.sinks);
-        auto hidden = [&](int key) {
-          return !(key <= pos && key < r.kv_end && (p.window == 0 || key > pos - p.window || key < p.sinks));
+        // which of 32 keys the row sees, one bit a key
+        auto visible = [&](int key) {
+          auto below = [&](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };  // keys before key + n
+          uint32_t m = below(min(pos + 1, r.kv_end) - key);
+          if (p.window > 0) m &= ~below(pos - p.window + 1 - key) | below(p.sinks - key);
+          return m;
         };
         const float4* sc = S.scale[st];
         lvs_top = fmaxf(lvs_top, sc[0].w);
-        // the tile's maximum
+        // the tile's maximum (loops kept short: the softmax warps' code has to stay in the
+        // instruction caches beside the other roles')
         float top = kNone;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float s[32];
           tc::ld32_wait(t_s + 32 * c, s);
           if (!open) {
+            const uint32_t m = visible(key0 + 32 * c);
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (hidden(key0 + 32 * c + k)) s[k] = -INFINITY;
+            for (int k = 0; k < 32; ++k) s[k] = m >> k & 1 ? s[k] : -INFINITY;
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -591,29 +599,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         first = false;
         // P, 32 keys at a time, over the scores already read
-        float sv[2][32];
-        tc::ld32(t_s, sv[0]);
-        tc::wait_ld(sv[0]);
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          float(&s)[32] = sv[c & 1];
-          if (c < 3) tc::ld32(t_s + 32 * (c + 1), sv[(c + 1) & 1]);
-          float pk[16];
+          float s[32], pk[16];
+          tc::ld32_wait(t_s + 32 * c, s);
+          if (!open) {
+            const uint32_t m = visible(key0 + 32 * c);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) s[k] = m >> k & 1 ? s[k] : -INFINITY;
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float4 f = sc[(32 * c + 16 * h) >> p.shift];
-            const float mul = coef * f.x, add = f.y - ref;
+            const float mul = fmaxf(coef * f.x, kTiny), add = f.y - ref;
             float* y = s + 16 * h;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) y[k] = fmaf(y[k], mul, add);
-            if (!open) {
-#pragma unroll
-              for (int k = 0; k < 16; ++k)
-                if (hidden(key0 + 32 * c + 16 * h + k)) y[k] = -INFINITY;
-            }
             uint32_t e[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
+              y[2 * k] = fmaf(y[2 * k], mul, add);
+              y[2 * k + 1] = fmaf(y[2 * k + 1], mul, add);
               e[k] = ex2_h2(pack_h2(y[2 * k], y[2 * k + 1]));
               pk[8 * h + k] = __uint_as_float(e[k]);
             }
@@ -631,7 +635,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           tc::st(t_s + 16 * c, pk);
-          if (c < 3) tc::wait_ld(sv[(c + 1) & 1]);
         }
         tc::wait_st();
         tc::fence_before_sync();
