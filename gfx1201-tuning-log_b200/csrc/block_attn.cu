@@ -91,15 +91,23 @@ int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args*
   p.records = reinterpret_cast<int*>(ws + kCounterBytes);
   p.partials = reinterpret_cast<float*>(ws + kCounterBytes + kRecordBytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  CUtensorMap km, vm;
-  if (!encode_paged_kv(&km, c->k, kHead, (uint32_t)c->num_kv_heads, (uint32_t)c->block_size, (uint64_t)c->num_blocks,
-                       (uint64_t)c->sk2, (uint64_t)c->sk1, (uint64_t)c->sk0) ||
-      !encode_paged_kv(&vm, c->v, kHead, (uint32_t)c->num_kv_heads, (uint32_t)c->block_size, (uint64_t)c->num_blocks,
-                       (uint64_t)c->sv2, (uint64_t)c->sv1, (uint64_t)c->sv0))
-    return B200KV_ERR_UNSUPPORTED;
   const int64_t rows = (int64_t)a->max_qlen * p.group;
+  auto maps = [&](CUtensorMap* km, CUtensorMap* vm, int box_tokens) {
+    return encode_paged_kv(km, c->k, kHead, (uint32_t)c->num_kv_heads, (uint32_t)c->block_size,
+                           (uint64_t)c->num_blocks, (uint64_t)c->sk2, (uint64_t)c->sk1, (uint64_t)c->sk0,
+                           (uint32_t)box_tokens) &&
+           encode_paged_kv(vm, c->v, kHead, (uint32_t)c->num_kv_heads, (uint32_t)c->block_size,
+                           (uint64_t)c->num_blocks, (uint64_t)c->sv2, (uint64_t)c->sv1, (uint64_t)c->sv0,
+                           (uint32_t)box_tokens);
+  };
+  CUtensorMap km, vm;
+  if (!maps(&km, &vm, c->block_size)) return B200KV_ERR_UNSUPPORTED;
   cudaError_t e = cudaSuccess;
-  if (rows > kMaxRows) e = block_prefill_launch(km, vm, p, st);
+  if (rows > kMaxRows) {
+    CUtensorMap km64 = km, vm64 = vm;
+    if (c->block_size > 64 && !maps(&km64, &vm64, 64)) return B200KV_ERR_UNSUPPORTED;
+    e = block_prefill_launch(km64, vm64, p, st);
+  }
   if (e == cudaSuccess) e = block_decode_launch(km, vm, p, rows < kMaxRows ? (int)rows : kMaxRows, st);
   return e == cudaSuccess ? B200KV_OK : B200KV_ERR_LAUNCH;
 }

@@ -60,19 +60,20 @@ struct BlockAttnParams {
   int* records;     // [kMaxCtas][8]: the many-query kernel's cut items, for the join after it
 };
 
-// The 128-key tiles that the queries at positions first .. see, of keys [0, kv_end):
-// tiles 0 .. sinks - 1, then low ..
+// The tiles of 2^SHIFT keys that the queries at positions first .. see, of keys
+// [0, kv_end): tiles 0 .. sinks - 1, then low ..
 struct KeyTiles {
   int sinks, low, count;
   __device__ __forceinline__ int tile(int j) const { return j < sinks ? j : low + j - sinks; }
 };
+template <int SHIFT>
 __device__ __forceinline__ KeyTiles key_tiles(const BlockAttnParams& p, int first, int kv_end) {
   KeyTiles t = {0, 0, 0};
   if (kv_end <= 0) return t;
-  const int high = (kv_end - 1) / 128 + 1;
+  const int high = ((kv_end - 1) >> SHIFT) + 1;
   if (p.window > 0) {
-    t.low = min(max(0, first - p.window + 1) / 128, high);
-    t.sinks = p.sinks > 0 ? min((min(p.sinks, kv_end) - 1) / 128 + 1, t.low) : 0;
+    t.low = min(max(0, first - p.window + 1) >> SHIFT, high);
+    t.sinks = p.sinks > 0 ? min(((min(p.sinks, kv_end) - 1) >> SHIFT) + 1, t.low) : 0;
   }
   t.count = t.sinks + high - t.low;
   return t;
@@ -94,7 +95,7 @@ int block_attn_shares(BlockAttnParams* p);
 // sequences with at most kMaxRows rows per kv head; `rows` bounds them in this batch
 cudaError_t block_decode_launch(const CUtensorMap& km, const CUtensorMap& vm, BlockAttnParams p, int rows,
                                 cudaStream_t st);
-// the others
+// the others; the maps' boxes hold min(block size, 64) tokens
 cudaError_t block_prefill_launch(const CUtensorMap& km, const CUtensorMap& vm, BlockAttnParams p, cudaStream_t st);
 
 }  // namespace b200kv

@@ -158,7 +158,7 @@ __device__ __forceinline__ Span span_of(const BlockAttnParams& p, int seq, int m
   s.q0 = s.total - s.qlen;
   s.kv_end = min(s.total, p.max_blocks << p.shift);
   s.keys.count = 0;
-  if (s.qlen > 0 && s.qlen <= max_rows && s.qlen * p.group <= max_rows) s.keys = key_tiles(p, s.q0, s.kv_end);
+  if (s.qlen > 0 && s.qlen <= max_rows && s.qlen * p.group <= max_rows) s.keys = key_tiles<7>(p, s.q0, s.kv_end);
   return s;
 }
 

@@ -15,17 +15,21 @@
 // Block scales ks, vs as in block_decode.cu: x = sm_scale log2(e) ks (q . k) + log2(vs),
 // P = 2^(x - m), and the softmax sum adds P / vs.  A softmax thread is a query row:
 // it finds the tile's maximum of x (the block's raw maximum, then the scale), moves m
-// when it is passed by 2^4, and then forms P in f16 pairs.  P <= 2^4.  The sum of a
-// block is taken in f16 pairs and joined in fp32; where a block's scale is below
-// 2^-10 of the largest seen, whose P may underflow though its weight P / vs does
-// not, the sum is formed from fp32 exponentials.
+// when it is passed by 2^4, and then forms P <= 2^4, in fp32 for the sum (where a
+// small block scale makes P small though its weight P / vs is not), rounded to f16
+// for the product.
 //
 // Shares of the batch's tiles as in block_decode.cu, an item being the two query
 // tiles of a kv head; what a cut item's shares leave is joined by a second kernel.
 //
-// Roles: 8 softmax warps (four a query tile), 4 that convert V, an MMA warp a query
-// tile (each waits for its own P V before its next Q K^T, which overwrites P: the
-// other tile's products fill the gap), a TMA warp, a warp for the blocks' scales.
+// Tiles are 64 keys, so that tensor memory holds two score tiles of each query tile
+// (4 x 64 columns) beside the two outputs (2 x 128): while the softmax works on one,
+// the next is multiplied, and P V and the Q K^T that reuses its columns leave the
+// softmax's chain.  Shared memory then has room for the next item's Q as well.
+//
+// Roles: 8 softmax warps (four a query tile, a thread a row), 2 that convert V, 2 that
+// lay out Q, a warp a query tile that issues its products, a TMA warp, a warp for the
+// blocks' scales.
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -43,34 +47,39 @@ namespace b200kv {
 namespace {
 
 constexpr int kHead = 128;
-constexpr int kTile = 128;               // keys of a tile, rows of a query tile
-constexpr int kBytes8 = kTile * kHead;   // an 8-bit operand
-constexpr int kKStages = 3, kVStages = 2, kScStages = 4;
-constexpr int kMaxPages = 8;
-constexpr int kSoftWarps = 8, kConvWarp = 8, kConvWarps = 4, kMmaWarp = 12, kTmaWarp = 14, kScaleWarp = 15;
+constexpr int kRows = 128;               // of a query tile
+constexpr int kShift = 6, kTile = 64;    // keys of a tile
+constexpr int kBytesQ = kRows * kHead;   // a term of Q
+constexpr int kBytes8 = kTile * kHead;   // K or V codes of a tile, and half the dimensions of its V in f16
+constexpr int kKStages = 3, kV8Stages = 2, kV16Stages = 3, kScStages = 4;
+constexpr int kMaxPages = 4;
+constexpr int kSoftWarps = 8, kConvWarp = 8, kConvWarps = 2, kQWarp = 10, kQWarps = 2, kMmaWarp = 12;
+constexpr int kTmaWarp = 14, kScaleWarp = 15;
 constexpr int kThreads = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 4.f;
-constexpr float kFar = 10.f;             // log2 of how far apart blocks' scales may be for f16 sums
 constexpr float kMinScale = 8.2718061e-25f, kMaxScale = 1.2089258e24f;  // 2^-80, 2^80
 constexpr float kNone = -1e30f;          // the reference of a row that has seen no key
+constexpr int kPoly = 3;                 // of eight pairs of a row's scores, those whose exponentials are polynomials
 constexpr float kTiny = 1e-37f;          // a factor of zero becomes it, so that a hidden key stays -inf
 
 // shared memory
-constexpr int kOffQ = 0;                          // [query tile][hi, lo]
-constexpr int kOffK = kOffQ + 4 * kBytes8;
+constexpr int kOffQ = 0;                          // [segment parity][query tile][hi, lo]
+constexpr int kOffK = kOffQ + 8 * kBytesQ;
 constexpr int kOffV8 = kOffK + kKStages * kBytes8;
-constexpr int kOffV16 = kOffV8 + kVStages * kBytes8;  // [stage][dims 0-63, 64-127][key][128 B]
-constexpr int kSmem = kOffV16 + kVStages * 2 * kBytes8;
+constexpr int kOffV16 = kOffV8 + kV8Stages * kBytes8;  // [stage][dims 0-63, 64-127][key][128 B]
+constexpr int kSmem = kOffV16 + kV16Stages * 2 * kBytes8;
 
 struct Shared {
   uint64_t k_full[kKStages], k_empty[kKStages];
-  uint64_t v8_full[kVStages], v8_empty[kVStages], v16_full[kVStages], v16_empty[kVStages];
+  uint64_t v8_full[kV8Stages], v8_empty[kV8Stages], v16_full[kV16Stages], v16_empty[kV16Stages];
   uint64_t sc_full[kScStages], sc_empty[kScStages];
-  uint64_t q_full[2], q_free[2], s_full[2], p_full[2], pv_done[2];
+  uint64_t q_full[2], q_free[2];                     // [segment parity]
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [query tile][tile parity]
   uint32_t tmem;
-  alignas(16) float4 scale[kScStages][kMaxPages];  // ks, log2 vs, 1 / vs, the tile's largest log2 vs
-  int first[4];                                    // of this share: sequence, head of the CTA's, pair, tile
+  float factor[2][2][kRows];                         // [segment parity][query tile] score factors
+  alignas(16) float4 scale[kScStages][kMaxPages];    // ks, log2 vs, 1 / vs
+  int first[4];                                      // of this share: sequence, head of the CTA's, pair, tile
   int warp_sum[kThreads / 32];
 };
 
@@ -94,7 +103,7 @@ __device__ __forceinline__ Seq seq_of(const BlockAttnParams& p, int seq) {
   const int total = p.lens[seq];
   s.q0 = total - s.qlen;
   s.kv_end = min(total, p.max_blocks << p.shift);
-  const int tokens = kTile / p.group;
+  const int tokens = kRows / p.group;
   const bool many = s.qlen > kMaxRows || s.qlen * p.group > kMaxRows;
   s.pairs = many ? (s.qlen - 1) / (2 * tokens) + 1 : 0;
   return s;
@@ -105,17 +114,22 @@ __device__ __forceinline__ Pair pair_of(const BlockAttnParams& p, const Seq& s, 
   r.qlen = s.qlen;
   r.q0 = s.q0;
   r.kv_end = s.kv_end;
-  r.tokens = kTile / p.group;
+  r.tokens = kRows / p.group;
   r.t0 = pair * 2 * r.tokens;
-  r.keys = key_tiles(p, s.q0 + r.t0, min(s.kv_end, s.q0 + min(s.qlen, r.t0 + 2 * r.tokens)));
+  r.keys = key_tiles<kShift>(p, s.q0 + r.t0, min(s.kv_end, s.q0 + min(s.qlen, r.t0 + 2 * r.tokens)));
   return r;
 }
-// whether no query of tile X sees key tile t
-__device__ __forceinline__ bool skips(const BlockAttnParams& p, const Pair& r, int X, int t) {
-  const int lo = t * kTile, first = r.first(X), last = r.last(X);
-  return last < first || lo > last || lo >= r.kv_end ||
-         (p.window > 0 && lo + kTile - 1 <= first - p.window && lo >= p.sinks);
-}
+// The key tiles of a pair that a query of tile X sees.
+struct Cut {
+  int lo, hi, sinks;
+  __device__ __forceinline__ Cut(const BlockAttnParams& p, const Pair& r, int X) {
+    const int first = r.first(X), last = r.last(X);
+    hi = last < first ? -1 : min(last, r.kv_end - 1) >> kShift;
+    lo = p.window > 0 ? max(0, first - p.window + 1) >> kShift : 0;
+    sinks = (p.sinks + kTile - 1) >> kShift;
+  }
+  __device__ __forceinline__ bool skips(int t) const { return t > hi || (t < lo && t >= sinks); }
+};
 
 // A CTA's share, segment by segment.
 struct Walk {
@@ -164,22 +178,49 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {  // a in the low
   asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ uint32_t ex2_h2(uint32_t x) {
-  uint32_t y;
-  asm("ex2.approx.f16x2 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t add_h2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+// pairs of floats, and their packed arithmetic
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float sum_h2(uint32_t x) {
+__device__ __forceinline__ void unpair2(uint64_t x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2_(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
   float a, b;
-  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.f32.f16 %0, l;\n cvt.f32.f16 %1, h;\n}"
-      : "=f"(a), "=f"(b)
-      : "r"(x));
-  return a + b;
+  unpair2(x, a, b);
+  return pair2(ex2(a), ex2(b));
+}
+// 2^x for x in [-126, 127] without the exponential unit, which serves a warp in eight
+// cycles and would bound the kernel alone: x = n + f with n the nearest whole number
+// (the sum with 1.5 2^23 leaves n in the low bits), 2^f by the cubic of least relative
+// error on [-1/2, 1/2] (7.5e-5, below the f16 rounding of P), and n added to its
+// exponent.  Below -126: 2^-126.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+  float a, b;
+  unpair2(x, a, b);
+  x = pair2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t t = add2_(x, pair2(12582912.f, 12582912.f));
+  const uint64_t f = fma2(add2_(t, pair2(-12582912.f, -12582912.f)), pair2(-1.f, -1.f), x);
+  uint64_t y = fma2(f, pair2(0.05517167f, 0.05517167f), pair2(0.24261113f, 0.24261113f));
+  y = fma2(y, f, pair2(0.69326097f, 0.69326097f));
+  y = fma2(y, f, pair2(0.99992806f, 0.99992806f));
+  float ta, tb, ya, yb;
+  unpair2(t, ta, tb);
+  unpair2(y, ya, yb);
+  return pair2(__int_as_float(__float_as_int(ya) + (__float_as_int(ta) << 23)),
+               __int_as_float(__float_as_int(yb) + (__float_as_int(tb) << 23)));
 }
 // two e4m3 codes (bytes 2 s, 2 s + 1 of w) -> f16x2 of 2^-8 their values
 template <int S>
@@ -202,9 +243,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&S.k_full[s], 1);
       mbar_init(&S.k_empty[s], 2);  // one arrival a query tile
     }
-    for (int s = 0; s < kVStages; ++s) {
+    for (int s = 0; s < kV8Stages; ++s) {
       mbar_init(&S.v8_full[s], 1);
       mbar_init(&S.v8_empty[s], kConvWarps);
+    }
+    for (int s = 0; s < kV16Stages; ++s) {
       mbar_init(&S.v16_full[s], kConvWarps);
       mbar_init(&S.v16_empty[s], 2);
     }
@@ -213,11 +256,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&S.sc_empty[s], kSoftWarps);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&S.q_full[b], 4);
-      mbar_init(&S.q_free[b], 1);
-      mbar_init(&S.s_full[b], 1);
-      mbar_init(&S.p_full[b], 4);
-      mbar_init(&S.pv_done[b], 1);
+      mbar_init(&S.q_full[b], kQWarps);
+      mbar_init(&S.q_free[b], 2 + kSoftWarps);  // issuers and softmax warps at a segment's end
+      for (int X = 0; X < 2; ++X) {
+        mbar_init(&S.s_full[X][b], 1);
+        mbar_init(&S.p_full[X][b], 4);
+        mbar_init(&S.pv_done[X][b], 1);
+      }
     }
     fence_mbar_init();
   }
@@ -279,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
   }
   __syncthreads();
-  const uint32_t tbase = S.tmem;  // S (then P) of tile 0, 1, O of tile 0, 1: 128 columns each
+  const uint32_t tbase = S.tmem;  // two score tiles (then P) of query tile 0, of 1, O of 0, of 1: 128 columns each
 
   if (warp == kScaleWarp) {
     // queries that see no key and whose pair has none: zeros
@@ -299,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!busy) {
   } else if (warp == kTmaWarp) {
     // ---------------- TMA producer ------------------------------------------------------
-    const int ppt = kTile >> p.shift, bs = 1 << p.shift, tpw = 32 / ppt;
+    const int bs = min(1 << p.shift, kTile), ppt = kTile / bs, tpw = 32 / ppt;  // boxes of bs tokens
     if (lane == 0) {
       tma_prefetch_desc(&kmap);
       tma_prefetch_desc(&vmap);
@@ -307,64 +352,67 @@ __global__ void __launch_bounds__(kThreads, 1)
     int i = 0;
     bool ok = true;
     for (Walk w(p, S, begin, count); w.left > 0 && ok; w.next()) {
-      const int n = w.count(), kh = w.kh();
+      const int n = w.count(), kh = w.kh(), kv_end = w.r.kv_end;
       const int32_t* row = p.bt + (int64_t)w.seq * p.bt_stride;
+      auto key_of = [&](int j0) { return w.r.keys.tile(w.off + j0 + lane / ppt) * kTile + lane % ppt * bs; };
       auto entry = [&](int j0) {
-        const int j = j0 + lane / ppt;
-        if (j >= n) return -1;
-        const int page = w.r.keys.tile(w.off + j) * ppt + lane % ppt;
-        return page << p.shift < w.r.kv_end ? __ldg(row + page) : -1;
+        if (j0 + lane / ppt >= n) return -1;
+        const int key = key_of(j0);
+        return key < kv_end ? __ldg(row + (key >> p.shift)) : -1;
       };
       int cur = entry(0), nxt = entry(tpw);
       for (int j = 0; j < n; ++j, ++i) {
-        const int ks = i % kKStages, vs = i % kVStages, j0 = j % tpw;
+        const int ks = i % kKStages, vs = i % kV8Stages, j0 = j % tpw;
         if (j > 0 && j0 == 0) {
           cur = nxt;
           nxt = entry(j + tpw);
         }
-        const int keys = min(kTile, w.r.kv_end - w.r.keys.tile(w.off + j) * kTile);
-        const int pages = (keys + bs - 1) >> p.shift;
-        const int pg = lane - j0 * ppt;
-        const bool mine = pg >= 0 && pg < pages;
+        const int key0 = w.r.keys.tile(w.off + j) * kTile;
+        const int boxes = (min(kTile, kv_end - key0) + bs - 1) / bs;
+        const int box = lane - j0 * ppt;
+        const bool mine = box >= 0 && box < boxes;
+        const int slot0 = (key0 + box * bs) & ((1 << p.shift) - 1);  // the box's first token in its block
         int free = 1;
         if (lane == 0 && i >= kKStages) free = mbar_wait_bounded(&S.k_empty[ks], (i / kKStages - 1) & 1);
         if (!__shfl_sync(0xffffffffu, free, 0)) {
           ok = false;
           break;
         }
-        if (lane == 0) mbar_arrive_expect_tx(&S.k_full[ks], (uint32_t)(pages * bs * kHead));
+        if (lane == 0) mbar_arrive_expect_tx(&S.k_full[ks], (uint32_t)(boxes * bs * kHead));
         __syncwarp();
-        if (mine) tma_load_4d(smem + kOffK + ks * kBytes8 + pg * bs * kHead, &kmap, 0, kh, 0, cur, &S.k_full[ks]);
-        if (lane == 0 && i >= kVStages) free = mbar_wait_bounded(&S.v8_empty[vs], (i / kVStages - 1) & 1);
+        if (mine)
+          tma_load_4d(smem + kOffK + ks * kBytes8 + box * bs * kHead, &kmap, 0, kh, slot0, cur, &S.k_full[ks]);
+        if (lane == 0 && i >= kV8Stages) free = mbar_wait_bounded(&S.v8_empty[vs], (i / kV8Stages - 1) & 1);
         if (!__shfl_sync(0xffffffffu, free, 0)) {
           // K of this tile is in flight, V is not: the consumers' waits give up too
           if (lane == 0) mbar_wait_bounded(&S.k_full[ks], (i / kKStages) & 1);
           ok = false;
           break;
         }
-        if (lane == 0) mbar_arrive_expect_tx(&S.v8_full[vs], (uint32_t)(pages * bs * kHead));
+        if (lane == 0) mbar_arrive_expect_tx(&S.v8_full[vs], (uint32_t)(boxes * bs * kHead));
         __syncwarp();
-        if (mine) tma_load_4d(smem + kOffV8 + vs * kBytes8 + pg * bs * kHead, &vmap, 0, kh, 0, cur, &S.v8_full[vs]);
+        if (mine)
+          tma_load_4d(smem + kOffV8 + vs * kBytes8 + box * bs * kHead, &vmap, 0, kh, slot0, cur, &S.v8_full[vs]);
       }
     }
     if (lane == 0) {  // every copy issued has landed before the CTA may exit
       for (int j = max(0, i - kKStages); j < i; ++j) mbar_wait_bounded(&S.k_full[j % kKStages], (j / kKStages) & 1);
-      for (int j = max(0, i - kVStages); j < i; ++j) mbar_wait_bounded(&S.v8_full[j % kVStages], (j / kVStages) & 1);
+      for (int j = max(0, i - kV8Stages); j < i; ++j) mbar_wait_bounded(&S.v8_full[j % kV8Stages], (j / kV8Stages) & 1);
     }
     __syncwarp();
   } else if (warp == kScaleWarp) {
     // ---------------- the blocks' scales ------------------------------------------------
-    const int ppt = kTile >> p.shift;
+    const int sub = min(p.shift, kShift), ppt = kTile >> sub;  // one entry a block, or for all of a tile
     int i = 0;
     bool failed = false;
     for (Walk w(p, S, begin, count); w.left > 0; w.next()) {
       const int n = w.count(), kh = w.kh();
       const int32_t* row = p.bt + (int64_t)w.seq * p.bt_stride;
-      auto load = [&](int j) {  // this lane's page of tile j
+      auto load = [&](int j) {  // this lane's block of tile j
         float2 v = make_float2(0.f, 0.f);
-        const int page = j < n ? w.r.keys.tile(w.off + j) * ppt + lane : 0;
-        if (j < n && lane < ppt && page << p.shift < w.r.kv_end) {
-          const int blk = __ldg(row + page);
+        const int key = j < n && lane < ppt ? w.r.keys.tile(w.off + j) * kTile + (lane << sub) : w.r.kv_end;
+        if (key < w.r.kv_end) {
+          const int blk = __ldg(row + (key >> p.shift));
           if (blk >= 0 && blk < p.num_blocks)  // else the block reads as zeros
             v = make_float2(p.ks[(int64_t)blk * p.ks0 + (int64_t)kh * p.ks1], p.vs[(int64_t)blk * p.vs0 + (int64_t)kh * p.vs1]);
         }
@@ -376,13 +424,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float2 v = nxt;
         nxt = load(j + 1);
         const float vs = fminf(fmaxf(v.y, kMinScale), kMaxScale);
-        const float lvs = __log2f(vs);
-        const bool real = lane < ppt && (w.r.keys.tile(w.off + j) * ppt + lane) << p.shift < w.r.kv_end;
-        float top = real ? lvs : -100.f;
-#pragma unroll
-        for (int o = 1; o < kMaxPages; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (i >= kScStages && !failed) failed = !mbar_wait_bounded(&S.sc_empty[st], (i / kScStages - 1) & 1);
-        if (lane < ppt) S.scale[st][lane] = make_float4(v.x, lvs, __frcp_rn(vs), top);
+        if (lane < ppt) S.scale[st][lane] = make_float4(v.x, __log2f(vs), __frcp_rn(vs), 0.f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.sc_full[st]);
       }
@@ -390,73 +433,87 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp >= kMmaWarp && warp < kMmaWarp + 2) {
     // ---------------- the products of one query tile --------------------------------------
     if (lane == 0) {
-      constexpr uint32_t kIdescQK = tc::idesc_f16_f32(kTile, kTile, false);
-      constexpr uint32_t kIdescPV = tc::idesc_f16_f32(kTile, kHead, true);
+      constexpr uint32_t kIdescQK = tc::idesc_f16_f32(kRows, kTile, false);
+      constexpr uint32_t kIdescPV = tc::idesc_f16_f32(kRows, kHead, true);
       const int X = warp - kMmaWarp;
-      const uint32_t a_q = smem_u32(smem + kOffQ + 2 * X * kBytes8), a_k = smem_u32(smem + kOffK);
-      const uint32_t a_v = smem_u32(smem + kOffV16), t_s = tbase + X * kTile, t_o = tbase + 2 * kTile + X * kTile;
+      const uint32_t a_k = smem_u32(smem + kOffK), a_v = smem_u32(smem + kOffV16);
+      const uint32_t t_s = tbase + X * kRows, t_o = tbase + 2 * kRows + X * kRows;
       bool failed = false;
-      int i = 0, done = 0, seg = 0;  // done: tiles of this query tile
+      int i0 = 0, qk = 0, pv = 0, seg = 0;  // qk, pv: products of this query tile so far
       for (Walk w(p, S, begin, count); w.left > 0; w.next(), ++seg) {
-        const int n = w.count();
-        if (!failed) failed = !mbar_wait_bounded(&S.q_full[X], seg & 1);
+        const int n = w.count(), off = w.off;
+        const KeyTiles keys = w.r.keys;
+        const Cut cut(p, w.r, X);
+        const uint32_t a_q = smem_u32(smem + kOffQ + (4 * (seg & 1) + 2 * X) * kBytesQ);
+        if (!failed) failed = !mbar_wait_bounded(&S.q_full[seg & 1], (seg >> 1) & 1);
         bool first = true;
-        for (int j = 0; j < n; ++j, ++i) {
-          const int ks = i % kKStages, vs = i % kVStages;
-          if (skips(p, w.r, X, w.r.keys.tile(w.off + j))) {
-            // the tile's buffers are released once they have been filled, so that no
-            // arrival runs ahead of its phase
+        int jq = 0, jp = 0;  // the tiles whose products with Q, with P come next
+        for (;;) {
+          while (jq < n && qk - pv < 2) {
+            const int i = i0 + jq, ks = i % kKStages;
+            const bool skip = cut.skips(keys.tile(off + jq));
+            if (skip && qk != pv) break;  // first the products before it: it releases its V too
             if (!failed) failed = !mbar_wait_bounded(&S.k_full[ks], (i / kKStages) & 1);
-            mbar_arrive(&S.k_empty[ks]);
-            if (!failed) failed = !mbar_wait_bounded(&S.v16_full[vs], (i / kVStages) & 1);
-            mbar_arrive(&S.v16_empty[vs]);
-            continue;
+            if (skip) {  // its buffers are released once filled, so that no arrival runs ahead of its phase
+              const int vs = i % kV16Stages;
+              if (!failed) failed = !mbar_wait_bounded(&S.v16_full[vs], (i / kV16Stages) & 1);
+              mbar_arrive(&S.k_empty[ks]);
+              mbar_arrive(&S.v16_empty[vs]);
+              jp = ++jq;
+              continue;
+            }
+            if (!failed) {
+              tc::fence_after_sync();
+#pragma unroll
+              for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                  tc::mma_f8(t_s + (qk & 1) * kTile, tc::sdesc_sw128(a_q + t * kBytesQ + d * 32, 16, 1024),
+                             tc::sdesc_sw128(a_k + ks * kBytes8 + d * 32, 16, 1024), kIdescQK, (t | d) != 0);
+            }
+            tc::commit(&S.s_full[X][qk & 1]);
+            tc::commit(&S.k_empty[ks]);
+            ++qk;
+            ++jq;
           }
-          if (!failed) failed = !mbar_wait_bounded(&S.k_full[ks], (i / kKStages) & 1);
+          if (qk == pv) break;  // the segment's products are done
+          const int i = i0 + jp, vs = i % kV16Stages, b = pv & 1;
+          if (!failed) failed = !mbar_wait_bounded(&S.v16_full[vs], (i / kV16Stages) & 1);
+          if (!failed) failed = !mbar_wait_bounded(&S.p_full[X][b], (pv >> 1) & 1);
           if (!failed) {
             tc::fence_after_sync();
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-              for (int d = 0; d < 4; ++d)
-                tc::mma_f8(t_s, tc::sdesc_sw128(a_q + t * kBytes8 + d * 32, 16, 1024),
-                           tc::sdesc_sw128(a_k + ks * kBytes8 + d * 32, 16, 1024), kIdescQK, (t | d) != 0);
+            for (int c = 0; c < kTile / 16; ++c)
+              tc::mma_f16_ts(t_o, t_s + b * kTile + 8 * c,
+                             tc::sdesc_sw128(a_v + vs * 2 * kBytes8 + c * 16 * 128, kBytes8, 1024), kIdescPV,
+                             !first || c != 0);
           }
-          tc::commit(&S.s_full[X]);
-          tc::commit(&S.k_empty[ks]);
-          if (!failed) failed = !mbar_wait_bounded(&S.p_full[X], done & 1);
-          if (!failed) failed = !mbar_wait_bounded(&S.v16_full[vs], (i / kVStages) & 1);
-          if (!failed) {
-            tc::fence_after_sync();
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              tc::mma_f16_ts(t_o, t_s + 8 * c, tc::sdesc_sw128(a_v + vs * 2 * kBytes8 + c * 16 * 128, kBytes8, 1024),
-                             kIdescPV, !first || c != 0);
-          }
-          tc::commit(&S.pv_done[X]);
+          tc::commit(&S.pv_done[X][b]);
           tc::commit(&S.v16_empty[vs]);
-          // the next Q K^T overwrites P
-          if (!failed) failed = !mbar_wait_bounded(&S.pv_done[X], done & 1);
+          // the score tile after the next overwrites this P
+          if (!failed) failed = !mbar_wait_bounded(&S.pv_done[X][b], (pv >> 1) & 1);
           first = false;
-          ++done;
+          ++pv;
+          ++jp;
         }
-        mbar_arrive(&S.q_free[X]);
+        mbar_arrive(&S.q_free[seg & 1]);
+        i0 += n;
       }
     }
     __syncwarp();
   } else if (warp >= kConvWarp && warp < kConvWarp + kConvWarps) {
     // ---------------- V codes to f16 ----------------------------------------------------
-    const int ct = tid - kConvWarp * 32, c = ct & 7;  // 16 codes, dims 16 c .., of keys ct / 8 + 16 e
+    const int ct = tid - kConvWarp * 32, c = ct & 7;  // 16 codes, dims 16 c .., of keys ct / 8 + 8 e
     bool failed = false;
     for (int i = 0; i < count; ++i) {
-      const int st = i % kVStages;
-      if (!failed) failed = !mbar_wait_bounded(&S.v8_full[st], (i / kVStages) & 1);
-      if (i >= kVStages && !failed) failed = !mbar_wait_bounded(&S.v16_empty[st], (i / kVStages - 1) & 1);
-      const uint8_t* src = smem + kOffV8 + st * kBytes8;
+      const int s8 = i % kV8Stages, st = i % kV16Stages;
+      if (!failed) failed = !mbar_wait_bounded(&S.v8_full[s8], (i / kV8Stages) & 1);
+      if (i >= kV16Stages && !failed) failed = !mbar_wait_bounded(&S.v16_empty[st], (i / kV16Stages - 1) & 1);
+      const uint8_t* src = smem + kOffV8 + s8 * kBytes8;
       uint8_t* dst = smem + kOffV16 + st * 2 * kBytes8 + (c >> 2) * kBytes8;
-#pragma unroll
+#pragma unroll 4
       for (int e = 0; e < 8; ++e) {
-        const int key = ct / 8 + 16 * e;
+        const int key = ct / 8 + 8 * e;
         const uint4 v = *reinterpret_cast<const uint4*>(src + swz(key, c));
         const uint4 a = make_uint4(half2_of<0>(v.x), half2_of<1>(v.x), half2_of<0>(v.y), half2_of<1>(v.y));
         const uint4 b = make_uint4(half2_of<0>(v.z), half2_of<1>(v.z), half2_of<0>(v.w), half2_of<1>(v.w));
@@ -468,84 +525,100 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&S.v8_empty[st]);
+        mbar_arrive(&S.v8_empty[s8]);
         mbar_arrive(&S.v16_full[st]);
       }
+    }
+  } else if (warp >= kQWarp && warp < kQWarp + kQWarps) {
+    // ---------------- Q of the segments, one ahead ----------------------------------------
+    // A power-of-two prescale a row (maximum in [2^7, 2^8)) with the sign of sm_scale, two
+    // terms; eight lanes a row.
+    const int qt = tid - kQWarp * 32, c = qt & 7;
+    bool failed = false;
+    int seg = 0;
+    for (Walk w(p, S, begin, count); w.left > 0; w.next(), ++seg) {
+      const int b = seg & 1, kh = w.kh();
+      const Pair& r = w.r;
+      if (seg >= 2 && !failed) failed = !mbar_wait_bounded(&S.q_free[b], ((seg >> 1) - 1) & 1);
+      for (int e = 0; e < 2 * kRows / (4 * kQWarps) / 4; ++e) {  // four rows a thread at a time
+        uint4 raw[4][2];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int a = qt / 8 + 4 * kQWarps * (4 * e + u), X = a / kRows, row = a % kRows;
+          const int t = r.t0 + X * r.tokens + row / p.group;
+          const bool valid = row < r.tokens * p.group && t < r.qlen;
+          const uint4* src = reinterpret_cast<const uint4*>(
+              p.q + (int64_t)(r.row0 + (valid ? t : 0)) * p.q_st + (int64_t)(kh * p.group + row % p.group) * p.q_sh +
+              16 * c);
+          raw[u][0] = valid ? __ldg(src) : make_uint4(0, 0, 0, 0);
+          raw[u][1] = valid ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int a = qt / 8 + 4 * kQWarps * (4 * e + u), X = a / kRows, row = a % kRows;
+          float v[16], mx = 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t x[4] = {raw[u][h].x, raw[u][h].y, raw[u][h].z, raw[u][h].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              v[8 * h + 2 * k] = __uint_as_float(x[k] << 16);
+              v[8 * h + 2 * k + 1] = __uint_as_float(x[k] & 0xFFFF0000u);
+              mx = fmaxf(mx, fmaxf(fabsf(v[8 * h + 2 * k]), fabsf(v[8 * h + 2 * k + 1])));
+            }
+          }
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const int E = (int)((__float_as_uint(mx) >> 23) & 0xFF);
+          int sh = (E == 0xFF || mx == 0.f) ? 0 : 134 - E;
+          sh = max(-126, min(126, sh));
+          const float up = __uint_as_float((uint32_t)(sh + 127) << 23 | (p.sm_scale < 0.f ? 0x80000000u : 0u));
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] *= up;
+          uint4 hi, lo;
+          pack16<1>(v, hi, lo);
+          uint8_t* q = smem + kOffQ + (4 * b + 2 * X) * kBytesQ;
+          *reinterpret_cast<uint4*>(q + swz(row, c)) = hi;
+          *reinterpret_cast<uint4*>(q + kBytesQ + swz(row, c)) = lo;
+          if (c == 0)
+            S.factor[b][X][row] = fabsf(p.sm_scale) * kLog2e * __uint_as_float((uint32_t)(127 - sh) << 23);
+        }
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.q_full[b]);
     }
   } else if (warp < kSoftWarps) {
     // ---------------- softmax: a thread is a query row ------------------------------------
     const int X = warp >> 2, row = tid & 127;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tbase + X * kTile + lane_off, t_o = tbase + 2 * kTile + X * kTile + lane_off;
+    const uint32_t t_o = tbase + 2 * kRows + X * kRows + lane_off;
     bool failed = false;
-    int i = 0, done = 0, seg = 0;
+    int i = 0, done = 0, seg = 0;  // done: tiles of this query tile so far
     for (Walk w(p, S, begin, count); w.left > 0; w.next(), ++seg) {
-      const int n = w.count(), kh = w.kh();
+      const int n = w.count(), kh = w.kh(), off = w.off;
+      const int64_t item = w.item;
       const Pair& r = w.r;
+      const Cut cut(p, r, X);
       const int t = r.t0 + X * r.tokens + row / p.group;
       const bool valid = row < r.tokens * p.group && t < r.qlen;
       const int pos = valid ? r.q0 + t : r.last(X);
-      const int64_t q_row = r.row0 + (valid ? t : 0);
-      const int head = kh * p.group + row % p.group;
-      float coef;
-      // the issuer is through with the segment before (one whose tiles this query tile
-      // skips would else let these warps run ahead of its barriers)
-      if (seg > 0 && !failed) failed = !mbar_wait_bounded(&S.q_free[X], (seg - 1) & 1);
-      {
-        // Q: a power-of-two prescale (maximum in [2^7, 2^8)) with the sign of sm_scale, two
-        // terms; the row is read twice, the second time from L1
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + q_row * p.q_st + (int64_t)head * p.q_sh);
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        float mx = 0.f;
-#pragma unroll 4
-        for (int c = 0; c < 16; ++c) {
-          const uint4 w4 = valid ? __ldg(src + c) : zero;
-          const uint32_t u[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(u[k] << 16)), fabsf(__uint_as_float(u[k] & 0xFFFF0000u))));
-        }
-        const int E = (int)((__float_as_uint(mx) >> 23) & 0xFF);
-        int sh = (E == 0xFF || mx == 0.f) ? 0 : 134 - E;
-        sh = max(-126, min(126, sh));
-        float up = __uint_as_float((uint32_t)(sh + 127) << 23);
-        if (p.sm_scale < 0.f) up = -up;
-        uint8_t* q = smem + kOffQ + 2 * X * kBytes8;
-#pragma unroll 1
-        for (int c = 0; c < 8; ++c) {
-          float v[16];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 w4 = valid ? __ldg(src + 2 * c + h) : zero;
-            const uint32_t u[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              v[8 * h + 2 * k] = __uint_as_float(u[k] << 16) * up;
-              v[8 * h + 2 * k + 1] = __uint_as_float(u[k] & 0xFFFF0000u) * up;
-            }
-          }
-          uint4 hi, lo;
-          pack16<1>(v, hi, lo);
-          *reinterpret_cast<uint4*>(q + swz(row, c)) = hi;
-          *reinterpret_cast<uint4*>(q + kBytes8 + swz(row, c)) = lo;
-        }
-        coef = fabsf(p.sm_scale) * kLog2e * __uint_as_float((uint32_t)(127 - sh) << 23);
-      }
-      tc::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&S.q_full[X]);
+      if (!failed) failed = !mbar_wait_bounded(&S.q_full[seg & 1], (seg >> 1) & 1);
+      const float coef = S.factor[seg & 1][X][row];
 
-      float ref = kNone, l = 0.f, lvs_top = -100.f;
+      float ref = kNone, l = 0.f;
       bool first = true;
       for (int j = 0; j < n; ++j, ++i) {
-        const int st = i % kScStages, tile = r.keys.tile(w.off + j), key0 = tile * kTile;
+        const int st = i % kScStages, tile = r.keys.tile(off + j), key0 = tile * kTile;
         if (!failed) failed = !mbar_wait_bounded(&S.sc_full[st], (i / kScStages) & 1);
-        if (skips(p, r, X, tile)) {
+        if (cut.skips(tile)) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&S.sc_empty[st]);
           continue;
         }
-        if (!failed) failed = !mbar_wait_bounded(&S.s_full[X], done & 1);
+        const int b = done & 1;
+        const uint32_t t_s = tbase + X * kRows + b * kTile + lane_off;  // its scores, and its P over them
+        if (!failed) failed = !mbar_wait_bounded(&S.s_full[X][b], (done >> 1) & 1);
         tc::fence_after_sync();
         const bool open = key0 + kTile - 1 <= r.first(X) && key0 + kTile <= r.kv_end &&
                           (p.window == 0 || key0 > r.last(X) - p.window || key0 + kTile <= p.sinks);
@@ -557,12 +630,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           return m;
         };
         const float4* sc = S.scale[st];
-        lvs_top = fmaxf(lvs_top, sc[0].w);
         // the tile's maximum (loops kept short: the softmax warps' code has to stay in the
         // instruction caches beside the other roles')
         float top = kNone;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           float s[32];
           tc::ld32_wait(t_s + 32 * c, s);
           if (!open) {
@@ -585,7 +657,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float now = moves ? top : ref, alpha = ex2(ref - now);
           ref = now;
           l *= alpha;
-          if (!first) {  // the product before this tile's is done: its issuer waited for it
+          if (!first) {
+            // the product before this tile's is done
+            if (!failed) failed = !mbar_wait_bounded(&S.pv_done[X][b ^ 1], ((done - 1) >> 1) & 1);
+            tc::fence_after_sync();
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               float o[32];
@@ -600,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         first = false;
         // P, 32 keys at a time, over the scores already read
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           float s[32], pk[16];
           tc::ld32_wait(t_s + 32 * c, s);
           if (!open) {
@@ -613,26 +688,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float4 f = sc[(32 * c + 16 * h) >> p.shift];
             const float mul = fmaxf(coef * f.x, kTiny), add = f.y - ref;
             float* y = s + 16 * h;
-            uint32_t e[8];
+            const uint64_t mul2 = pair2(mul, mul), add2 = pair2(add, add);
+            uint64_t sum2[2] = {0, 0};
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              y[2 * k] = fmaf(y[2 * k], mul, add);
-              y[2 * k + 1] = fmaf(y[2 * k + 1], mul, add);
-              e[k] = ex2_h2(pack_h2(y[2 * k], y[2 * k + 1]));
-              pk[8 * h + k] = __uint_as_float(e[k]);
+              const uint64_t x = fma2(pair2(y[2 * k], y[2 * k + 1]), mul2, add2);
+              const uint64_t e = k % 8 < kPoly ? exp2_poly(x) : exp2_mufu(x);
+              sum2[k & 1] = add2_(sum2[k & 1], e);
+              float u, v;
+              unpair2(e, u, v);
+              pk[8 * h + k] = __uint_as_float(pack_h2(u, v));
             }
-            if (f.y > lvs_top - kFar) {  // uniform over the CTA
-#pragma unroll
-              for (int o = 4; o > 0; o >>= 1)
-#pragma unroll
-                for (int k = 0; k < o; ++k) e[k] = add_h2(e[k], e[k + o]);
-              l = fmaf(sum_h2(e[0]), f.z, l);
-            } else {
-              float sum = 0.f;
-#pragma unroll
-              for (int k = 0; k < 16; ++k) sum += ex2(y[k]);
-              l = fmaf(sum, f.z, l);
-            }
+            float sa, sb;
+            unpair2(add2_(sum2[0], sum2[1]), sa, sb);
+            l = fmaf(sa + sb, f.z, l);
           }
           tc::st(t_s + 16 * c, pk);
         }
@@ -641,19 +710,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&S.sc_empty[st]);
-          mbar_arrive(&S.p_full[X]);
+          mbar_arrive(&S.p_full[X][b]);
         }
         ++done;
       }
 
       // ---- the segment's end ----------------------------------------------------------------
       const bool whole = n == r.keys.count;
-      float* part = p.partials + (int64_t)(2 * blockIdx.x + (w.item >= begin ? 1 : 0)) * kPartialFloats;
-      if (!first && !failed) failed = !mbar_wait_bounded(&S.pv_done[X], (done - 1) & 1);
+      float* part = p.partials + (int64_t)(2 * blockIdx.x + (item >= begin ? 1 : 0)) * kPartialFloats;
+      if (!first && !failed) failed = !mbar_wait_bounded(&S.pv_done[X][(done - 1) & 1], ((done - 1) >> 1) & 1);
       tc::fence_after_sync();
       const float f = whole ? (l > 0.f ? __fdividef(256.f, l) : 0.f) : 256.f;  // V entered as 2^-8 V
-      __nv_bfloat16* dst = p.out + q_row * p.o_st + (int64_t)head * p.o_sh;
-      float* pdst = part + (X * kTile + row) * kHead;
+      __nv_bfloat16* dst =
+          p.out + (int64_t)(r.row0 + (valid ? t : 0)) * p.o_st + (int64_t)(kh * p.group + row % p.group) * p.o_sh;
+      float* pdst = part + (X * kRows + row) * kHead;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         float o[32];
@@ -683,16 +753,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!whole && valid)
-        *reinterpret_cast<float2*>(part + kPairRows * kHead + 2 * (X * kTile + row)) = make_float2(ref, l);
-      if (!whole && w.item >= begin && tid == 0) {  // the item begins here and is cut: what its join needs
+        *reinterpret_cast<float2*>(part + kPairRows * kHead + 2 * (X * kRows + row)) = make_float2(ref, l);
+      if (!whole && item >= begin && tid == 0) {  // the item begins here and is cut: what its join needs
         int* rec = p.records + blockIdx.x * 8;
         rec[1] = r.row0;
         rec[2] = r.qlen;
         rec[3] = r.t0;
         rec[4] = kh;
-        rec[5] = share_owner(w.item + r.keys.count - 1, total, shares);
+        rec[5] = share_owner(item + r.keys.count - 1, total, shares);
         rec[0] = 1;
       }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.q_free[seg & 1]);
     }
   }
   tc::fence_before_sync();
@@ -709,10 +782,10 @@ __global__ void __launch_bounds__(128) block_prefill_join_kernel(const BlockAttn
   const int* rec = p.records + blockIdx.x * 8;
   if (!rec[0]) return;
   const int row0 = rec[1], qlen = rec[2], t0 = rec[3], kh = rec[4], c_hi = rec[5];
-  const int slot = blockIdx.x % p.slots, c_lo = blockIdx.x / p.slots, tokens = kTile / p.group;
+  const int slot = blockIdx.x % p.slots, c_lo = blockIdx.x / p.slots, tokens = kRows / p.group;
   for (int e = threadIdx.x; e < kJoinRows * (kHead / 4); e += 128) {
     const int a = blockIdx.y * kJoinRows + e / (kHead / 4), c = e % (kHead / 4);
-    const int X = a / kTile, row = a % kTile, t = t0 + X * tokens + row / p.group;
+    const int X = a / kRows, row = a % kRows, t = t0 + X * tokens + row / p.group;
     if (row >= tokens * p.group || t >= qlen) continue;
     float top = kNone, sum = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);

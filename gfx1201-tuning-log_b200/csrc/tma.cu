@@ -56,13 +56,13 @@ bool encode_e2m1_unpacked_2d(CUtensorMap* map, const void* base, uint64_t row_el
 
 bool encode_paged_kv(CUtensorMap* map, const void* base, uint32_t row_bytes, uint32_t heads,
                      uint32_t tokens, uint64_t blocks, uint64_t s_head, uint64_t s_tok,
-                     uint64_t s_blk) {
+                     uint64_t s_blk, uint32_t box_tokens) {
   PFN_cuTensorMapEncodeTiled enc = get_encode();
   if (!enc || row_bytes != 128 || tokens == 0 || tokens > 256 || blocks == 0) return false;
   if ((s_head | s_tok | s_blk) & 15) return false;
   const cuuint64_t dims[4] = {row_bytes, heads, tokens, blocks};
   const cuuint64_t strides[3] = {s_head, s_tok, s_blk};
-  const cuuint32_t box[4] = {row_bytes, 1, tokens, 1};
+  const cuuint32_t box[4] = {row_bytes, 1, box_tokens ? box_tokens : tokens, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims,
                          strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

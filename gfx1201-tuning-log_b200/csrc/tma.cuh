@@ -43,9 +43,10 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
 // load brings one head's rows of one page into shared memory as a swizzled
 // [tokens][row_bytes] tile.  row_bytes must be 128.  Out-of-range block ids
 // read as zeros.
+// box_tokens (0: all of the page's): tokens of a box, starting at any token of the page.
 bool encode_paged_kv(CUtensorMap* map, const void* base, uint32_t row_bytes, uint32_t heads,
                      uint32_t tokens, uint64_t blocks, uint64_t s_head, uint64_t s_tok,
-                     uint64_t s_blk);
+                     uint64_t s_blk, uint32_t box_tokens = 0);
 
 
 // 4-D tiled TMA load of the box at (c0 bytes, c1, c2, c3), completion counted on
