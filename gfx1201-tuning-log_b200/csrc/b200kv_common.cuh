@@ -107,6 +107,27 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   return false;
 }
 
+// The same wait, parked: the hardware may suspend the warp for up to a millisecond a
+// poll, so that the waiting warps of a kernel of many roles do not take issue slots
+// from its working ones (the block-scaled prefill: 20 % of its time).
+__device__ __forceinline__ bool mbar_wait_parked(uint64_t* bar, uint32_t parity, uint32_t max_tries = 4096) {
+  const uint32_t addr = smem_u32(bar);
+#pragma unroll 1
+  for (uint32_t i = 0; i < max_tries; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(addr), "r"(parity), "r"(1000000u)
+        : "memory");
+    if (done) return true;
+  }
+  atomicExch(&g_device_status, kDevMbarrierTimeout);
+  return false;
+}
+
 // Global nanosecond timer (bounded spins on flags in global memory).
 __device__ __forceinline__ unsigned long long globaltimer_ns() {
   unsigned long long t;

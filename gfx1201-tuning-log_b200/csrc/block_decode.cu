@@ -187,6 +187,7 @@ struct Walk {
     off = 0;
     if (++sub == p.heads) {
       sub = 0;
+#pragma unroll 1
       do {
         s = span_of(p, ++seq, max_rows);
       } while (s.keys.count == 0 && seq + 1 < p.num_seqs);
@@ -209,6 +210,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
 
   if (tid == 0) {
     griddep_launch_dependents();
+#pragma unroll 1
     for (int s = 0; s < NS; ++s) {
       mbar_init(&S.kv_full[s], 2 * (1 + 32));  // K's and V's bytes, and each producer lane's scales
       mbar_init(&S.kv_empty[s], 1);
@@ -231,6 +233,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
   const int per = (p.num_seqs + kThreads - 1) / kThreads;
   const int s_lo = min(p.num_seqs, tid * per), s_hi = min(p.num_seqs, s_lo + per);
   int mine = 0;
+#pragma unroll 1
   for (int s = s_lo; s < s_hi; ++s) mine += span_of(p, s, R).keys.count;
   int incl = mine;
 #pragma unroll
@@ -257,6 +260,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
   if (busy) {
     int at = before + incl - mine;  // tiles of the sequences before this thread's
     if (begin >= (int64_t)at * p.heads && begin < (int64_t)(at + mine) * p.heads)
+#pragma unroll 1
       for (int s = s_lo; s < s_hi; ++s) {
         const int n = span_of(p, s, R).keys.count;
         if (begin < (int64_t)(at + n) * p.heads) {
@@ -272,9 +276,11 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
 
   if (warp == SH::kPvWarp) {  // it waits for the first P anyway
     // queries of sequences without a key: zeros
+#pragma unroll 1
     for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
       const Span sp = span_of(p, s, R);
       if (sp.keys.count == 0 && sp.qlen > 0 && sp.qlen <= R && sp.qlen * p.group <= R)
+#pragma unroll 1
         for (int i = lane; i < sp.qlen * p.hkv * p.group * kHead; i += 32) {
           const int t = i / (p.hkv * p.group * kHead), h = i / kHead % (p.hkv * p.group);
           p.out[(int64_t)(sp.row0 + t) * p.o_st + (int64_t)h * p.o_sh + i % kHead] = __float2bfloat16_rn(0.f);
@@ -293,6 +299,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
     if (lane == 0) tma_prefetch_desc(map);
     int i = 0;
     bool ok = true;
+#pragma unroll 1
     for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0 && ok; w.next()) {
       const int n = w.count(), kh = w.kh();
       const int32_t* row = p.bt + (int64_t)w.seq * p.bt_stride;
@@ -303,6 +310,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
         return page << p.shift < w.s.kv_end ? __ldg(row + page) : -1;
       };
       int cur = entry(0), nxt = entry(tpw);
+#pragma unroll 1
       for (int j = 0; j < n; ++j, ++i) {
         const int st = i % NS, j0 = j % tpw;
         if (j > 0 && j0 == 0) {
@@ -310,7 +318,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
           nxt = entry(j + tpw);
         }
         int free = 1;
-        if (lane == 0 && i >= NS) free = mbar_wait_bounded(&S.kv_empty[st], (i / NS - 1) & 1);
+        if (lane == 0 && i >= NS) free = mbar_wait_parked(&S.kv_empty[st], (i / NS - 1) & 1);
         if (!__shfl_sync(0xffffffffu, free, 0)) {
           ok = false;
           break;
@@ -330,7 +338,8 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
     }
     // every copy issued has landed before the CTA may exit
     if (lane == 0)
-      for (int j = max(0, i - NS); j < i; ++j) mbar_wait_bounded(&S.kv_full[j % NS], (j / NS) & 1);
+#pragma unroll 1
+      for (int j = max(0, i - NS); j < i; ++j) mbar_wait_parked(&S.kv_full[j % NS], (j / NS) & 1);
     __syncwarp();
   } else if (warp == SH::kQkWarp) {
     // ---------------- S^T = K Q^T -------------------------------------------------------
@@ -339,12 +348,14 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
       const uint32_t a_kv = smem_u32(smem), a_q = smem_u32(smem + SH::kOffQ);
       bool failed = false;
       int i = 0, seg = 0;
+#pragma unroll 1
       for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0; w.next(), ++seg) {
-        if (!failed) failed = !mbar_wait_bounded(&S.q_full[seg & 1], (seg >> 1) & 1);
+        if (!failed) failed = !mbar_wait_parked(&S.q_full[seg & 1], (seg >> 1) & 1);
+#pragma unroll 1
         for (int j = w.count(); j > 0; --j, ++i) {
           const int st = i % NS, b = i % LK;
-          if (!failed) failed = !mbar_wait_bounded(&S.kv_full[st], (i / NS) & 1);
-          if (i >= LK && !failed) failed = !mbar_wait_bounded(&S.s_free[b], (i / LK - 1) & 1);
+          if (!failed) failed = !mbar_wait_parked(&S.kv_full[st], (i / NS) & 1);
+          if (i >= LK && !failed) failed = !mbar_wait_parked(&S.s_free[b], (i / LK - 1) & 1);
           if (!failed) {
             tc::fence_after_sync();
 #pragma unroll
@@ -364,11 +375,13 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
       const uint32_t a_kv = smem_u32(smem), a_p = smem_u32(smem + SH::kOffP);
       bool failed = false;
       int i = 0;
+#pragma unroll 1
       for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0; w.next()) {
         const int n = w.count();
+#pragma unroll 1
         for (int j = 0; j < n; ++j, ++i) {
           const int st = i % NS, X = i % G;
-          if (!failed) failed = !mbar_wait_bounded(&S.p_full[X], (i / G) & 1);
+          if (!failed) failed = !mbar_wait_parked(&S.p_full[X], (i / G) & 1);
           if (!failed) {
             tc::fence_after_sync();
 #pragma unroll
@@ -400,6 +413,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
     // per row (maximum in [2^7, 2^8)), two terms
     auto put_q = [&](const Span& s, int kh, int qb) {
       const int rows = s.qlen * p.group;
+#pragma unroll 1
       for (int e = tid; e < R * 8; e += kSoftThreads) {
         const int r = e >> 3, c = e & 7, t = r / p.group;
         uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
@@ -444,6 +458,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
     };
     Walk w(p, R, S.first_seq, S.first_prefix, begin, count);
     put_q(w.s, w.kh(), 0);
+#pragma unroll 1
     for (; w.left > 0; ++seg) {
       const int n = w.count(), qb = seg & 1, kh = w.kh();
       const Span s = w.s;
@@ -461,11 +476,12 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
       for (int r = 0; r < RT; ++r) l[r] = 0.f;
       const int first = (X + G - i0 % G) % G;  // the segment's first tile of this group
       int k = (i0 + first) / G;                // the group's tiles so far
+#pragma unroll 1
       for (int j = first; j < n; j += G, ++k) {
         const int i = i0 + j, st = i % NS;
         const int key0 = s.keys.tile(off + j) * kTile, key = key0 + kt;
         const uint32_t t_s = tbase + (i % LK) * N + lane_off + r0;
-        if (!failed) failed = !mbar_wait_bounded(&S.s_full[i % LK], (i / LK) & 1);
+        if (!failed) failed = !mbar_wait_parked(&S.s_full[i % LK], (i / LK) & 1);
         tc::fence_after_sync();
         // all rows see the whole tile, or the mask is asked
         const bool open = key0 + kTile - 1 <= s.q0 && key0 + kTile <= s.kv_end &&
@@ -503,7 +519,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
         if (lane == 0) mbar_arrive(&S.s_free[i % LK]);
         const bool move = named_bar_or(bar, 128, over > kOff + kLazy);
         // the group's previous product is done: P is free and O is stable
-        if (k > 0 && !failed) failed = !mbar_wait_bounded(&S.pv_done[X], (k - 1) & 1);
+        if (k > 0 && !failed) failed = !mbar_wait_parked(&S.pv_done[X], (k - 1) & 1);
         tc::fence_after_sync();
         if (move) {
 #pragma unroll
@@ -574,7 +590,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
 
       // ---- the segment's end: join the groups, store or leave a partial ------------------
       const bool own = first < n;
-      if (own && !failed) failed = !mbar_wait_bounded(&S.pv_done[X], (k - 1) & 1);
+      if (own && !failed) failed = !mbar_wait_parked(&S.pv_done[X], (k - 1) & 1);
       tc::fence_after_sync();
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
@@ -616,6 +632,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
       };
       const bool whole = n == s.keys.count;
       float* part_o = p.partials + (int64_t)(2 * blockIdx.x + (item >= begin ? 1 : 0)) * kPartialFloats;
+#pragma unroll 1
       for (int e = tid; e < rows * (kHead / 4); e += kSoftThreads) {
         const int a = e / (kHead / 4), c = e % (kHead / 4);
         const float4 o = *reinterpret_cast<const float4*>(join + a * kHead + 4 * c);
@@ -648,10 +665,12 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
           constexpr int kJoin = R <= 16 ? 8 : 4;
           // later shares begin inside the item: it is their first
           const int at0 = item >= share_begin(c_lo, total, shares) ? 1 : 0;
+#pragma unroll 1
           for (int e = tid; e < rows * (kHead / 4); e += kSoftThreads) {
             const int a = e / (kHead / 4), c = e % (kHead / 4);
             float top = kNone, sum = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
             for (int c0 = c_lo; c0 <= c_hi; c0 += kJoin) {
               float2 ml[kJoin];
               float4 v[kJoin];

@@ -15,7 +15,7 @@
 // Block scales ks, vs as in block_decode.cu: x = sm_scale log2(e) ks (q . k) + log2(vs),
 // P = 2^(x - m), and the softmax sum adds P / vs.  A softmax thread is a query row:
 // it finds the tile's maximum of x (the block's raw maximum, then the scale), moves m
-// when it is passed by 2^4, and then forms P <= 2^4, in fp32 for the sum (where a
+// when it is passed by 2^8, and then forms P <= 2^8, in fp32 for the sum (where a
 // small block scale makes P small though its weight P / vs is not), rounded to f16
 // for the product.
 //
@@ -57,10 +57,9 @@ constexpr int kSoftWarps = 8, kConvWarp = 8, kConvWarps = 2, kQWarp = 10, kQWarp
 constexpr int kTmaWarp = 14, kScaleWarp = 15;
 constexpr int kThreads = 512;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazy = 4.f;
+constexpr float kLazy = 8.f;             // m moves when a maximum passes it by 2^8 (P stays within f16)
 constexpr float kMinScale = 8.2718061e-25f, kMaxScale = 1.2089258e24f;  // 2^-80, 2^80
 constexpr float kNone = -1e30f;          // the reference of a row that has seen no key
-constexpr int kPoly = 3;                 // of eight pairs of a row's scores, those whose exponentials are polynomials
 constexpr float kTiny = 1e-37f;          // a factor of zero becomes it, so that a hidden key stays -inf
 
 // shared memory
@@ -155,6 +154,7 @@ struct Walk {
     if (left <= 0) return;
     item += r.keys.count;
     off = 0;
+#pragma unroll 1
     do {
       if (++pair >= s.pairs) {
         pair = 0;
@@ -197,30 +197,10 @@ __device__ __forceinline__ uint64_t add2_(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
+__device__ __forceinline__ uint64_t exp2_2(uint64_t x) {
   float a, b;
   unpair2(x, a, b);
   return pair2(ex2(a), ex2(b));
-}
-// 2^x for x in [-126, 127] without the exponential unit, which serves a warp in eight
-// cycles and would bound the kernel alone: x = n + f with n the nearest whole number
-// (the sum with 1.5 2^23 leaves n in the low bits), 2^f by the cubic of least relative
-// error on [-1/2, 1/2] (7.5e-5, below the f16 rounding of P), and n added to its
-// exponent.  Below -126: 2^-126.
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
-  float a, b;
-  unpair2(x, a, b);
-  x = pair2(fmaxf(a, -126.f), fmaxf(b, -126.f));
-  const uint64_t t = add2_(x, pair2(12582912.f, 12582912.f));
-  const uint64_t f = fma2(add2_(t, pair2(-12582912.f, -12582912.f)), pair2(-1.f, -1.f), x);
-  uint64_t y = fma2(f, pair2(0.05517167f, 0.05517167f), pair2(0.24261113f, 0.24261113f));
-  y = fma2(y, f, pair2(0.69326097f, 0.69326097f));
-  y = fma2(y, f, pair2(0.99992806f, 0.99992806f));
-  float ta, tb, ya, yb;
-  unpair2(t, ta, tb);
-  unpair2(y, ya, yb);
-  return pair2(__int_as_float(__float_as_int(ya) + (__float_as_int(ta) << 23)),
-               __int_as_float(__float_as_int(yb) + (__float_as_int(tb) << 23)));
 }
 // two e4m3 codes (bytes 2 s, 2 s + 1 of w) -> f16x2 of 2^-8 their values
 template <int S>
@@ -239,18 +219,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     griddep_launch_dependents();
+#pragma unroll 1
     for (int s = 0; s < kKStages; ++s) {
       mbar_init(&S.k_full[s], 1);
       mbar_init(&S.k_empty[s], 2);  // one arrival a query tile
     }
+#pragma unroll 1
     for (int s = 0; s < kV8Stages; ++s) {
       mbar_init(&S.v8_full[s], 1);
       mbar_init(&S.v8_empty[s], kConvWarps);
     }
+#pragma unroll 1
     for (int s = 0; s < kV16Stages; ++s) {
       mbar_init(&S.v16_full[s], kConvWarps);
       mbar_init(&S.v16_empty[s], 2);
     }
+#pragma unroll 1
     for (int s = 0; s < kScStages; ++s) {
       mbar_init(&S.sc_full[s], 1);
       mbar_init(&S.sc_empty[s], kSoftWarps);
@@ -275,10 +259,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto seq_tiles = [&](int seq) {
     const Seq s = seq_of(p, seq);
     int n = 0;
+#pragma unroll 1
     for (int i = 0; i < s.pairs; ++i) n += pair_of(p, s, i).keys.count;
     return n;
   };
   int mine = 0;
+#pragma unroll 1
   for (int s = s_lo; s < s_hi; ++s) mine += seq_tiles(s);
   int incl = mine;
 #pragma unroll
@@ -306,6 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (busy) {
     int at = before + incl - mine;
     if (begin >= (int64_t)at * p.heads && begin < (int64_t)(at + mine) * p.heads)
+#pragma unroll 1
       for (int s = s_lo; s < s_hi; ++s) {
         const int n = seq_tiles(s);
         if (begin < (int64_t)(at + n) * p.heads) {
@@ -315,6 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           S.first[1] = rel / n;
           rel %= n;
           int pair = 0;
+#pragma unroll 1
           for (int m; rel >= (m = pair_of(p, q, pair).keys.count); ++pair) rel -= m;
           S.first[2] = pair;
           S.first[3] = rel;
@@ -328,13 +316,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == kScaleWarp) {
     // queries that see no key and whose pair has none: zeros
+#pragma unroll 1
     for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
       const Seq q = seq_of(p, s);
       if (q.pairs == 0 || (q.q0 >= 0 && q.kv_end > 0)) continue;
+#pragma unroll 1
       for (int i = 0; i < q.pairs; ++i) {
         const Pair r = pair_of(p, q, i);
         if (r.keys.count) continue;
         const int n = min(q.qlen - r.t0, 2 * r.tokens), width = p.hkv * p.group * kHead;
+#pragma unroll 1
         for (int64_t e = lane; e < (int64_t)n * width; e += 32)
           p.out[(int64_t)(q.row0 + r.t0 + e / width) * p.o_st + e % width / kHead * p.o_sh + e % kHead] =
               __float2bfloat16_rn(0.f);
@@ -351,6 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     int i = 0;
     bool ok = true;
+#pragma unroll 1
     for (Walk w(p, S, begin, count); w.left > 0 && ok; w.next()) {
       const int n = w.count(), kh = w.kh(), kv_end = w.r.kv_end;
       const int32_t* row = p.bt + (int64_t)w.seq * p.bt_stride;
@@ -361,6 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return key < kv_end ? __ldg(row + (key >> p.shift)) : -1;
       };
       int cur = entry(0), nxt = entry(tpw);
+#pragma unroll 1
       for (int j = 0; j < n; ++j, ++i) {
         const int ks = i % kKStages, vs = i % kV8Stages, j0 = j % tpw;
         if (j > 0 && j0 == 0) {
@@ -373,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool mine = box >= 0 && box < boxes;
         const int slot0 = (key0 + box * bs) & ((1 << p.shift) - 1);  // the box's first token in its block
         int free = 1;
-        if (lane == 0 && i >= kKStages) free = mbar_wait_bounded(&S.k_empty[ks], (i / kKStages - 1) & 1);
+        if (lane == 0 && i >= kKStages) free = mbar_wait_parked(&S.k_empty[ks], (i / kKStages - 1) & 1);
         if (!__shfl_sync(0xffffffffu, free, 0)) {
           ok = false;
           break;
@@ -382,10 +375,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (mine)
           tma_load_4d(smem + kOffK + ks * kBytes8 + box * bs * kHead, &kmap, 0, kh, slot0, cur, &S.k_full[ks]);
-        if (lane == 0 && i >= kV8Stages) free = mbar_wait_bounded(&S.v8_empty[vs], (i / kV8Stages - 1) & 1);
+        if (lane == 0 && i >= kV8Stages) free = mbar_wait_parked(&S.v8_empty[vs], (i / kV8Stages - 1) & 1);
         if (!__shfl_sync(0xffffffffu, free, 0)) {
           // K of this tile is in flight, V is not: the consumers' waits give up too
-          if (lane == 0) mbar_wait_bounded(&S.k_full[ks], (i / kKStages) & 1);
+          if (lane == 0) mbar_wait_parked(&S.k_full[ks], (i / kKStages) & 1);
           ok = false;
           break;
         }
@@ -396,8 +389,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (lane == 0) {  // every copy issued has landed before the CTA may exit
-      for (int j = max(0, i - kKStages); j < i; ++j) mbar_wait_bounded(&S.k_full[j % kKStages], (j / kKStages) & 1);
-      for (int j = max(0, i - kV8Stages); j < i; ++j) mbar_wait_bounded(&S.v8_full[j % kV8Stages], (j / kV8Stages) & 1);
+#pragma unroll 1
+      for (int j = max(0, i - kKStages); j < i; ++j) mbar_wait_parked(&S.k_full[j % kKStages], (j / kKStages) & 1);
+#pragma unroll 1
+      for (int j = max(0, i - kV8Stages); j < i; ++j) mbar_wait_parked(&S.v8_full[j % kV8Stages], (j / kV8Stages) & 1);
     }
     __syncwarp();
   } else if (warp == kScaleWarp) {
@@ -405,6 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int sub = min(p.shift, kShift), ppt = kTile >> sub;  // one entry a block, or for all of a tile
     int i = 0;
     bool failed = false;
+#pragma unroll 1
     for (Walk w(p, S, begin, count); w.left > 0; w.next()) {
       const int n = w.count(), kh = w.kh();
       const int32_t* row = p.bt + (int64_t)w.seq * p.bt_stride;
@@ -419,12 +415,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         return v;
       };
       float2 nxt = load(0);
+#pragma unroll 1
       for (int j = 0; j < n; ++j, ++i) {
         const int st = i % kScStages;
         const float2 v = nxt;
         nxt = load(j + 1);
         const float vs = fminf(fmaxf(v.y, kMinScale), kMaxScale);
-        if (i >= kScStages && !failed) failed = !mbar_wait_bounded(&S.sc_empty[st], (i / kScStages - 1) & 1);
+        if (i >= kScStages && !failed) failed = !mbar_wait_parked(&S.sc_empty[st], (i / kScStages - 1) & 1);
         if (lane < ppt) S.scale[st][lane] = make_float4(v.x, __log2f(vs), __frcp_rn(vs), 0.f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.sc_full[st]);
@@ -440,23 +437,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t t_s = tbase + X * kRows, t_o = tbase + 2 * kRows + X * kRows;
       bool failed = false;
       int i0 = 0, qk = 0, pv = 0, seg = 0;  // qk, pv: products of this query tile so far
+#pragma unroll 1
       for (Walk w(p, S, begin, count); w.left > 0; w.next(), ++seg) {
         const int n = w.count(), off = w.off;
         const KeyTiles keys = w.r.keys;
         const Cut cut(p, w.r, X);
         const uint32_t a_q = smem_u32(smem + kOffQ + (4 * (seg & 1) + 2 * X) * kBytesQ);
-        if (!failed) failed = !mbar_wait_bounded(&S.q_full[seg & 1], (seg >> 1) & 1);
+        if (!failed) failed = !mbar_wait_parked(&S.q_full[seg & 1], (seg >> 1) & 1);
         bool first = true;
         int jq = 0, jp = 0;  // the tiles whose products with Q, with P come next
+#pragma unroll 1
         for (;;) {
+#pragma unroll 1
           while (jq < n && qk - pv < 2) {
             const int i = i0 + jq, ks = i % kKStages;
             const bool skip = cut.skips(keys.tile(off + jq));
             if (skip && qk != pv) break;  // first the products before it: it releases its V too
-            if (!failed) failed = !mbar_wait_bounded(&S.k_full[ks], (i / kKStages) & 1);
+            if (!failed) failed = !mbar_wait_parked(&S.k_full[ks], (i / kKStages) & 1);
             if (skip) {  // its buffers are released once filled, so that no arrival runs ahead of its phase
               const int vs = i % kV16Stages;
-              if (!failed) failed = !mbar_wait_bounded(&S.v16_full[vs], (i / kV16Stages) & 1);
+              if (!failed) failed = !mbar_wait_parked(&S.v16_full[vs], (i / kV16Stages) & 1);
               mbar_arrive(&S.k_empty[ks]);
               mbar_arrive(&S.v16_empty[vs]);
               jp = ++jq;
@@ -478,8 +478,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (qk == pv) break;  // the segment's products are done
           const int i = i0 + jp, vs = i % kV16Stages, b = pv & 1;
-          if (!failed) failed = !mbar_wait_bounded(&S.v16_full[vs], (i / kV16Stages) & 1);
-          if (!failed) failed = !mbar_wait_bounded(&S.p_full[X][b], (pv >> 1) & 1);
+          if (!failed) failed = !mbar_wait_parked(&S.v16_full[vs], (i / kV16Stages) & 1);
+          if (!failed) failed = !mbar_wait_parked(&S.p_full[X][b], (pv >> 1) & 1);
           if (!failed) {
             tc::fence_after_sync();
 #pragma unroll
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::commit(&S.pv_done[X][b]);
           tc::commit(&S.v16_empty[vs]);
           // the score tile after the next overwrites this P
-          if (!failed) failed = !mbar_wait_bounded(&S.pv_done[X][b], (pv >> 1) & 1);
+          if (!failed) failed = !mbar_wait_parked(&S.pv_done[X][b], (pv >> 1) & 1);
           first = false;
           ++pv;
           ++jp;
@@ -505,10 +505,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- V codes to f16 ----------------------------------------------------
     const int ct = tid - kConvWarp * 32, c = ct & 7;  // 16 codes, dims 16 c .., of keys ct / 8 + 8 e
     bool failed = false;
+#pragma unroll 1
     for (int i = 0; i < count; ++i) {
       const int s8 = i % kV8Stages, st = i % kV16Stages;
-      if (!failed) failed = !mbar_wait_bounded(&S.v8_full[s8], (i / kV8Stages) & 1);
-      if (i >= kV16Stages && !failed) failed = !mbar_wait_bounded(&S.v16_empty[st], (i / kV16Stages - 1) & 1);
+      if (!failed) failed = !mbar_wait_parked(&S.v8_full[s8], (i / kV8Stages) & 1);
+      if (i >= kV16Stages && !failed) failed = !mbar_wait_parked(&S.v16_empty[st], (i / kV16Stages - 1) & 1);
       const uint8_t* src = smem + kOffV8 + s8 * kBytes8;
       uint8_t* dst = smem + kOffV16 + st * 2 * kBytes8 + (c >> 2) * kBytes8;
 #pragma unroll 4
@@ -536,10 +537,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int qt = tid - kQWarp * 32, c = qt & 7;
     bool failed = false;
     int seg = 0;
+#pragma unroll 1
     for (Walk w(p, S, begin, count); w.left > 0; w.next(), ++seg) {
       const int b = seg & 1, kh = w.kh();
       const Pair& r = w.r;
-      if (seg >= 2 && !failed) failed = !mbar_wait_bounded(&S.q_free[b], ((seg >> 1) - 1) & 1);
+      if (seg >= 2 && !failed) failed = !mbar_wait_parked(&S.q_free[b], ((seg >> 1) - 1) & 1);
+#pragma unroll 1
       for (int e = 0; e < 2 * kRows / (4 * kQWarps) / 4; ++e) {  // four rows a thread at a time
         uint4 raw[4][2];
 #pragma unroll
@@ -595,6 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_o = tbase + 2 * kRows + X * kRows + lane_off;
     bool failed = false;
     int i = 0, done = 0, seg = 0;  // done: tiles of this query tile so far
+#pragma unroll 1
     for (Walk w(p, S, begin, count); w.left > 0; w.next(), ++seg) {
       const int n = w.count(), kh = w.kh(), off = w.off;
       const int64_t item = w.item;
@@ -603,14 +607,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t = r.t0 + X * r.tokens + row / p.group;
       const bool valid = row < r.tokens * p.group && t < r.qlen;
       const int pos = valid ? r.q0 + t : r.last(X);
-      if (!failed) failed = !mbar_wait_bounded(&S.q_full[seg & 1], (seg >> 1) & 1);
+      if (!failed) failed = !mbar_wait_parked(&S.q_full[seg & 1], (seg >> 1) & 1);
       const float coef = S.factor[seg & 1][X][row];
 
       float ref = kNone, l = 0.f;
       bool first = true;
+#pragma unroll 1
       for (int j = 0; j < n; ++j, ++i) {
         const int st = i % kScStages, tile = r.keys.tile(off + j), key0 = tile * kTile;
-        if (!failed) failed = !mbar_wait_bounded(&S.sc_full[st], (i / kScStages) & 1);
+        if (!failed) failed = !mbar_wait_parked(&S.sc_full[st], (i / kScStages) & 1);
         if (cut.skips(tile)) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&S.sc_empty[st]);
@@ -618,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int b = done & 1;
         const uint32_t t_s = tbase + X * kRows + b * kTile + lane_off;  // its scores, and its P over them
-        if (!failed) failed = !mbar_wait_bounded(&S.s_full[X][b], (done >> 1) & 1);
+        if (!failed) failed = !mbar_wait_parked(&S.s_full[X][b], (done >> 1) & 1);
         tc::fence_after_sync();
         const bool open = key0 + kTile - 1 <= r.first(X) && key0 + kTile <= r.kv_end &&
                           (p.window == 0 || key0 > r.last(X) - p.window || key0 + kTile <= p.sinks);
@@ -659,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           l *= alpha;
           if (!first) {
             // the product before this tile's is done
-            if (!failed) failed = !mbar_wait_bounded(&S.pv_done[X][b ^ 1], ((done - 1) >> 1) & 1);
+            if (!failed) failed = !mbar_wait_parked(&S.pv_done[X][b ^ 1], ((done - 1) >> 1) & 1);
             tc::fence_after_sync();
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
@@ -693,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const uint64_t x = fma2(pair2(y[2 * k], y[2 * k + 1]), mul2, add2);
-              const uint64_t e = k % 8 < kPoly ? exp2_poly(x) : exp2_mufu(x);
+              const uint64_t e = exp2_2(x);
               sum2[k & 1] = add2_(sum2[k & 1], e);
               float u, v;
               unpair2(e, u, v);
@@ -718,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- the segment's end ----------------------------------------------------------------
       const bool whole = n == r.keys.count;
       float* part = p.partials + (int64_t)(2 * blockIdx.x + (item >= begin ? 1 : 0)) * kPartialFloats;
-      if (!first && !failed) failed = !mbar_wait_bounded(&S.pv_done[X][(done - 1) & 1], ((done - 1) >> 1) & 1);
+      if (!first && !failed) failed = !mbar_wait_parked(&S.pv_done[X][(done - 1) & 1], ((done - 1) >> 1) & 1);
       tc::fence_after_sync();
       const float f = whole ? (l > 0.f ? __fdividef(256.f, l) : 0.f) : 256.f;  // V entered as 2^-8 V
       __nv_bfloat16* dst =
@@ -790,6 +795,7 @@ __global__ void __launch_bounds__(128) block_prefill_join_kernel(const BlockAttn
     float top = kNone, sum = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int kFlight = 8;
+#pragma unroll 1
     for (int c0 = c_lo; c0 <= c_hi; c0 += kFlight) {
       float2 ml[kFlight];
       float4 v[kFlight];
