@@ -51,7 +51,8 @@ constexpr int kRows = 128;               // of a query tile
 constexpr int kShift = 6, kTile = 64;    // keys of a tile
 constexpr int kBytesQ = kRows * kHead;   // a term of Q
 constexpr int kBytes8 = kTile * kHead;   // K or V codes of a tile, and half the dimensions of its V in f16
-constexpr int kKStages = 3, kV8Stages = 2, kV16Stages = 3, kScStages = 4;
+constexpr int kKStages = 3, kV8Stages = 2, kV16Stages = 3;
+constexpr int kScales = 8;               // tiles whose blocks' scales are held: see the scale warp
 constexpr int kMaxPages = 4;
 constexpr int kSoftWarps = 8, kConvWarp = 8, kConvWarps = 2, kQWarp = 10, kQWarps = 2, kMmaWarp = 12;
 constexpr int kTmaWarp = 14, kScaleWarp = 15;
@@ -72,12 +73,11 @@ constexpr int kSmem = kOffV16 + kV16Stages * 2 * kBytes8;
 struct Shared {
   uint64_t k_full[kKStages], k_empty[kKStages];
   uint64_t v8_full[kV8Stages], v8_empty[kV8Stages], v16_full[kV16Stages], v16_empty[kV16Stages];
-  uint64_t sc_full[kScStages], sc_empty[kScStages];
   uint64_t q_full[2], q_free[2];                     // [segment parity]
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [query tile][tile parity]
   uint32_t tmem;
   float factor[2][2][kRows];                         // [segment parity][query tile] score factors
-  alignas(16) float4 scale[kScStages][kMaxPages];    // ks, log2 vs, 1 / vs
+  alignas(16) float4 scale[kScales][kMaxPages];    // ks, log2 vs, 1 / vs
   int first[4];                                      // of this share: sequence, head of the CTA's, pair, tile
   int warp_sum[kThreads / 32];
 };
@@ -178,6 +178,11 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {  // a in the low
   asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // pairs of floats, and their packed arithmetic
 __device__ __forceinline__ uint64_t pair2(float a, float b) {
   uint64_t r;
@@ -221,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     griddep_launch_dependents();
 #pragma unroll 1
     for (int s = 0; s < kKStages; ++s) {
-      mbar_init(&S.k_full[s], 1);
+      mbar_init(&S.k_full[s], 2);   // the bytes of K, and the scale warp
       mbar_init(&S.k_empty[s], 2);  // one arrival a query tile
     }
 #pragma unroll 1
@@ -235,10 +240,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&S.v16_empty[s], 2);
     }
 #pragma unroll 1
-    for (int s = 0; s < kScStages; ++s) {
-      mbar_init(&S.sc_full[s], 1);
-      mbar_init(&S.sc_empty[s], kSoftWarps);
-    }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&S.q_full[b], kQWarps);
       mbar_init(&S.q_free[b], 2 + kSoftWarps);  // issuers and softmax warps at a segment's end
@@ -417,14 +418,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       float2 nxt = load(0);
 #pragma unroll 1
       for (int j = 0; j < n; ++j, ++i) {
-        const int st = i % kScStages;
+        const int st = i % kScales, ks = i % kKStages;
         const float2 v = nxt;
         nxt = load(j + 1);
         const float vs = fminf(fmaxf(v.y, kMinScale), kMaxScale);
-        if (i >= kScStages && !failed) failed = !mbar_wait_parked(&S.sc_empty[st], (i / kScStages - 1) & 1);
+        // Once the stage of tile i - 3 is empty, both query tiles have had P of tile i - 5 and
+        // no softmax warp reads scales before tile i - 4's; the arrival counts for tile i.
+        if (i >= kKStages && !failed) failed = !mbar_wait_parked(&S.k_empty[ks], (i / kKStages - 1) & 1);
         if (lane < ppt) S.scale[st][lane] = make_float4(v.x, __log2f(vs), __frcp_rn(vs), 0.f);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&S.sc_full[st]);
+        if (lane == 0) mbar_arrive(&S.k_full[ks]);
       }
     }
   } else if (warp >= kMmaWarp && warp < kMmaWarp + 2) {
@@ -433,7 +436,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kIdescQK = tc::idesc_f16_f32(kRows, kTile, false);
       constexpr uint32_t kIdescPV = tc::idesc_f16_f32(kRows, kHead, true);
       const int X = warp - kMmaWarp;
-      const uint32_t a_k = smem_u32(smem + kOffK), a_v = smem_u32(smem + kOffV16);
+      // descriptors count 16 bytes in their low bits
+      const uint64_t d_k = tc::sdesc_sw128(smem_u32(smem + kOffK), 16, 1024);
+      const uint64_t d_v = tc::sdesc_sw128(smem_u32(smem + kOffV16), kBytes8, 1024);
       const uint32_t t_s = tbase + X * kRows, t_o = tbase + 2 * kRows + X * kRows;
       bool failed = false;
       int i0 = 0, qk = 0, pv = 0, seg = 0;  // qk, pv: products of this query tile so far
@@ -442,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = w.count(), off = w.off;
         const KeyTiles keys = w.r.keys;
         const Cut cut(p, w.r, X);
-        const uint32_t a_q = smem_u32(smem + kOffQ + (4 * (seg & 1) + 2 * X) * kBytesQ);
+        const uint64_t d_q = tc::sdesc_sw128(smem_u32(smem + kOffQ + (4 * (seg & 1) + 2 * X) * kBytesQ), 16, 1024);
         if (!failed) failed = !mbar_wait_parked(&S.q_full[seg & 1], (seg >> 1) & 1);
         bool first = true;
         int jq = 0, jp = 0;  // the tiles whose products with Q, with P come next
@@ -464,12 +469,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (!failed) {
               tc::fence_after_sync();
+              const uint64_t d_kt = d_k + ks * (kBytes8 / 16);
+              const uint32_t t_qk = t_s + (qk & 1) * kTile;
 #pragma unroll
               for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
-                  tc::mma_f8(t_s + (qk & 1) * kTile, tc::sdesc_sw128(a_q + t * kBytesQ + d * 32, 16, 1024),
-                             tc::sdesc_sw128(a_k + ks * kBytes8 + d * 32, 16, 1024), kIdescQK, (t | d) != 0);
+                  tc::mma_f8(t_qk, d_q + (t * kBytesQ + d * 32) / 16, d_kt + d * 2, kIdescQK, (t | d) != 0);
             }
             tc::commit(&S.s_full[X][qk & 1]);
             tc::commit(&S.k_empty[ks]);
@@ -482,11 +488,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!failed) failed = !mbar_wait_parked(&S.p_full[X][b], (pv >> 1) & 1);
           if (!failed) {
             tc::fence_after_sync();
+            const uint64_t d_vt = d_v + vs * (2 * kBytes8 / 16);
+            const uint32_t t_p = t_s + b * kTile;
 #pragma unroll
             for (int c = 0; c < kTile / 16; ++c)
-              tc::mma_f16_ts(t_o, t_s + b * kTile + 8 * c,
-                             tc::sdesc_sw128(a_v + vs * 2 * kBytes8 + c * 16 * 128, kBytes8, 1024), kIdescPV,
-                             !first || c != 0);
+              tc::mma_f16_ts(t_o, t_p + 8 * c, d_vt + c * 128, kIdescPV, !first || c != 0);
           }
           tc::commit(&S.pv_done[X][b]);
           tc::commit(&S.v16_empty[vs]);
@@ -614,13 +620,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool first = true;
 #pragma unroll 1
       for (int j = 0; j < n; ++j, ++i) {
-        const int st = i % kScStages, tile = r.keys.tile(off + j), key0 = tile * kTile;
-        if (!failed) failed = !mbar_wait_parked(&S.sc_full[st], (i / kScStages) & 1);
-        if (cut.skips(tile)) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&S.sc_empty[st]);
-          continue;
-        }
+        const int tile = r.keys.tile(off + j), key0 = tile * kTile;
+        if (cut.skips(tile)) continue;
         const int b = done & 1;
         const uint32_t t_s = tbase + X * kRows + b * kTile + lane_off;  // its scores, and its P over them
         if (!failed) failed = !mbar_wait_parked(&S.s_full[X][b], (done >> 1) & 1);
@@ -634,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (p.window > 0) m &= ~below(pos - p.window + 1 - key) | below(p.sinks - key);
           return m;
         };
-        const float4* sc = S.scale[st];
+        const float4* sc = S.scale[i % kScales];  // written before K's stage was full
         // the tile's maximum (loops kept short: the softmax warps' code has to stay in the
         // instruction caches beside the other roles')
         float top = kNone;
@@ -649,10 +650,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float m = s[16 * h];
-#pragma unroll
-            for (int k = 1; k < 15; k += 2) m = fmaxf(m, fmaxf(s[16 * h + k], s[16 * h + k + 1]));
-            m = fmaxf(m, s[16 * h + 15]);
+            const float* y = s + 16 * h;
+            float m = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), max3(y[6], y[7], y[8]));
+            m = max3(m, max3(y[9], y[10], y[11]), max3(y[12], y[13], max3(y[14], y[15], y[15])));
             const float4 f = sc[(32 * c + 16 * h) >> p.shift];
             if (m != -INFINITY) top = fmaxf(top, fmaf(m, coef * f.x, f.y));
           }
@@ -713,10 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::wait_st();
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&S.sc_empty[st]);
-          mbar_arrive(&S.p_full[X][b]);
-        }
+        if (lane == 0) mbar_arrive(&S.p_full[X][b]);
         ++done;
       }
 
