@@ -27,8 +27,8 @@
 // the next is multiplied, and P V and the Q K^T that reuses its columns leave the
 // softmax's chain.  Shared memory then has room for the next item's Q as well.
 //
-// Roles: 8 softmax warps (four a query tile, a thread a row), 2 that convert V, 2 that
-// lay out Q, a warp a query tile that issues its products, a TMA warp, a warp for the
+// Roles: 8 softmax warps (four a query tile, a thread a row), 2 that convert V, 6 that
+// lay out Q (with 2, prompts of 2048 tokens and less waited for it: 243 -> 162 us), a warp a query tile that issues its products, a TMA warp, a warp for the
 // blocks' scales.
 
 #include <cuda.h>
@@ -54,9 +54,9 @@ constexpr int kBytes8 = kTile * kHead;   // K or V codes of a tile, and half the
 constexpr int kKStages = 3, kV8Stages = 2, kV16Stages = 3;
 constexpr int kScales = 8;               // tiles whose blocks' scales are held: see the scale warp
 constexpr int kMaxPages = 4;
-constexpr int kSoftWarps = 8, kConvWarp = 8, kConvWarps = 2, kQWarp = 10, kQWarps = 2, kMmaWarp = 12;
-constexpr int kTmaWarp = 14, kScaleWarp = 15;
-constexpr int kThreads = 512;
+constexpr int kSoftWarps = 8, kConvWarp = 8, kConvWarps = 2, kQWarp = 10, kQWarps = 6, kMmaWarp = 16;
+constexpr int kTmaWarp = 18, kScaleWarp = 19;
+constexpr int kThreads = 640;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;             // m moves when a maximum passes it by 2^8 (P stays within f16)
 constexpr float kMinScale = 8.2718061e-25f, kMaxScale = 1.2089258e24f;  // 2^-80, 2^80
@@ -173,9 +173,21 @@ struct Walk {
   }
 };
 
+// row / group for row < 128, group <= 16: exact with the reciprocal rounded up
+__device__ __forceinline__ int over_group(int row, int inv) { return row * inv >> 16; }
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {  // a in the low half
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_abs_bf2(uint32_t a, uint32_t b) {  // larger magnitudes, of either sign
+  uint32_t r;
+  asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -313,6 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
   }
   __syncthreads();
+  const int inv_group = (65536 + p.group - 1) / p.group;
   const uint32_t tbase = S.tmem;  // two score tiles (then P) of query tile 0, of 1, O of 0, of 1: 128 columns each
 
   if (warp == kScaleWarp) {
@@ -472,10 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint64_t d_kt = d_k + ks * (kBytes8 / 16);
               const uint32_t t_qk = t_s + (qk & 1) * kTile;
 #pragma unroll
-              for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-                  tc::mma_f8(t_qk, d_q + (t * kBytesQ + d * 32) / 16, d_kt + d * 2, kIdescQK, (t | d) != 0);
+              for (int d = 0; d < 8; ++d)  // the first term of Q, then the second
+                tc::mma_f8(t_qk, d_q + (d >> 2) * (kBytesQ / 16) + (d & 3) * 2, d_kt + (d & 3) * 2, kIdescQK, d != 0);
             }
             tc::commit(&S.s_full[X][qk & 1]);
             tc::commit(&S.k_empty[ks]);
@@ -509,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp >= kConvWarp && warp < kConvWarp + kConvWarps) {
     // ---------------- V codes to f16 ----------------------------------------------------
-    const int ct = tid - kConvWarp * 32, c = ct & 7;  // 16 codes, dims 16 c .., of keys ct / 8 + 8 e
+    const int ct = tid - kConvWarp * 32, c = ct & 7;  // 16 codes, dims 16 c .., of every 4 kConvWarps-th key
     bool failed = false;
 #pragma unroll 1
     for (int i = 0; i < count; ++i) {
@@ -518,9 +529,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (i >= kV16Stages && !failed) failed = !mbar_wait_parked(&S.v16_empty[st], (i / kV16Stages - 1) & 1);
       const uint8_t* src = smem + kOffV8 + s8 * kBytes8;
       uint8_t* dst = smem + kOffV16 + st * 2 * kBytes8 + (c >> 2) * kBytes8;
-#pragma unroll 4
-      for (int e = 0; e < 8; ++e) {
-        const int key = ct / 8 + 8 * e;
+#pragma unroll 1
+      for (int key = ct / 8; key < kTile; key += 4 * kConvWarps) {
         const uint4 v = *reinterpret_cast<const uint4*>(src + swz(key, c));
         const uint4 a = make_uint4(half2_of<0>(v.x), half2_of<1>(v.x), half2_of<0>(v.y), half2_of<1>(v.y));
         const uint4 b = make_uint4(half2_of<0>(v.z), half2_of<1>(v.z), half2_of<0>(v.w), half2_of<1>(v.w));
@@ -548,50 +558,48 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int b = seg & 1, kh = w.kh();
       const Pair& r = w.r;
       if (seg >= 2 && !failed) failed = !mbar_wait_parked(&S.q_free[b], ((seg >> 1) - 1) & 1);
-#pragma unroll 1
-      for (int e = 0; e < 2 * kRows / (4 * kQWarps) / 4; ++e) {  // four rows a thread at a time
-        uint4 raw[4][2];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int a = qt / 8 + 4 * kQWarps * (4 * e + u), X = a / kRows, row = a % kRows;
-          const int t = r.t0 + X * r.tokens + row / p.group;
-          const bool valid = row < r.tokens * p.group && t < r.qlen;
+      uint4 n0, n1;  // the next row's chunk, in flight
+      auto load = [&](int a) {
+        const int X = a / kRows, row = a % kRows, tok = over_group(row, inv_group), t = r.t0 + X * r.tokens + tok;
+        n0 = n1 = make_uint4(0, 0, 0, 0);
+        if (a < 2 * kRows && tok < r.tokens && t < r.qlen) {
           const uint4* src = reinterpret_cast<const uint4*>(
-              p.q + (int64_t)(r.row0 + (valid ? t : 0)) * p.q_st + (int64_t)(kh * p.group + row % p.group) * p.q_sh +
-              16 * c);
-          raw[u][0] = valid ? __ldg(src) : make_uint4(0, 0, 0, 0);
-          raw[u][1] = valid ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+              p.q + (int64_t)(r.row0 + t) * p.q_st + (int64_t)(kh * p.group + row - tok * p.group) * p.q_sh + 16 * c);
+          n0 = __ldg(src);
+          n1 = __ldg(src + 1);
         }
+      };
+      load(qt / 8);
+#pragma unroll 1
+      for (int a = qt / 8; a < 2 * kRows; a += 4 * kQWarps) {
+        const int X = a / kRows, row = a % kRows;
+        const uint32_t w[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+        load(a + 4 * kQWarps);
+        uint32_t top = max_abs_bf2(max_abs_bf2(max_abs_bf2(w[0], w[1]), max_abs_bf2(w[2], w[3])),
+                                   max_abs_bf2(max_abs_bf2(w[4], w[5]), max_abs_bf2(w[6], w[7])));
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int a = qt / 8 + 4 * kQWarps * (4 * e + u), X = a / kRows, row = a % kRows;
-          float v[16], mx = 0.f;
+        for (int o = 1; o < 8; o <<= 1) top = max_abs_bf2(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const uint32_t mx = max(top & 0x7FFFu, top >> 16 & 0x7FFFu);  // bits of the row's largest magnitude
+        const int E = (int)(mx >> 7);
+        int sh = (E == 0xFF || mx == 0) ? 0 : 134 - E;
+        sh = max(-126, min(126, sh));
+        const float up = __uint_as_float((uint32_t)(sh + 127) << 23 | (p.sm_scale < 0.f ? 0x80000000u : 0u));
+        // hi: the magnitude rounded to 4 significant bits (half away from zero); the rest has
+        // at most 5 and is exact in bf16
+        uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t x[4] = {raw[u][h].x, raw[u][h].y, raw[u][h].z, raw[u][h].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              v[8 * h + 2 * k] = __uint_as_float(x[k] << 16);
-              v[8 * h + 2 * k + 1] = __uint_as_float(x[k] & 0xFFFF0000u);
-              mx = fmaxf(mx, fmaxf(fabsf(v[8 * h + 2 * k]), fabsf(v[8 * h + 2 * k + 1])));
-            }
-          }
-#pragma unroll
-          for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const int E = (int)((__float_as_uint(mx) >> 23) & 0xFF);
-          int sh = (E == 0xFF || mx == 0.f) ? 0 : 134 - E;
-          sh = max(-126, min(126, sh));
-          const float up = __uint_as_float((uint32_t)(sh + 127) << 23 | (p.sm_scale < 0.f ? 0x80000000u : 0u));
-#pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] *= up;
-          uint4 hi, lo;
-          pack16<1>(v, hi, lo);
-          uint8_t* q = smem + kOffQ + (4 * b + 2 * X) * kBytesQ;
-          *reinterpret_cast<uint4*>(q + swz(row, c)) = hi;
-          *reinterpret_cast<uint4*>(q + kBytesQ + swz(row, c)) = lo;
-          if (c == 0)
-            S.factor[b][X][row] = fabsf(p.sm_scale) * kLog2e * __uint_as_float((uint32_t)(127 - sh) << 23);
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t x = (w[k] + 0x00080008u) & 0xFFF0FFF0u, y = sub_bf2(w[k], x);
+          const uint32_t ch = e4m3x2(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xFFFF0000u) * up);
+          const uint32_t cl = e4m3x2(__uint_as_float(y << 16) * up, __uint_as_float(y & 0xFFFF0000u) * up);
+          hi[k / 2] = k & 1 ? hi[k / 2] | ch << 16 : ch;
+          lo[k / 2] = k & 1 ? lo[k / 2] | cl << 16 : cl;
         }
+        uint8_t* q = smem + kOffQ + (4 * b + 2 * X) * kBytesQ;
+        *reinterpret_cast<uint4*>(q + swz(row, c)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(q + kBytesQ + swz(row, c)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (c == 0)
+          S.factor[b][X][row] = fabsf(p.sm_scale) * kLog2e * __uint_as_float((uint32_t)(127 - sh) << 23);
       }
       tc::fence_proxy_async_smem();
       __syncwarp();
@@ -610,8 +618,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t item = w.item;
       const Pair& r = w.r;
       const Cut cut(p, r, X);
-      const int t = r.t0 + X * r.tokens + row / p.group;
-      const bool valid = row < r.tokens * p.group && t < r.qlen;
+      const int tok = over_group(row, inv_group), t = r.t0 + X * r.tokens + tok;
+      const bool valid = tok < r.tokens && t < r.qlen;
       const int pos = valid ? r.q0 + t : r.last(X);
       if (!failed) failed = !mbar_wait_parked(&S.q_full[seg & 1], (seg >> 1) & 1);
       const float coef = S.factor[seg & 1][X][row];
@@ -628,13 +636,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after_sync();
         const bool open = key0 + kTile - 1 <= r.first(X) && key0 + kTile <= r.kv_end &&
                           (p.window == 0 || key0 > r.last(X) - p.window || key0 + kTile <= p.sinks);
-        // which of 32 keys the row sees, one bit a key
-        auto visible = [&](int key) {
-          auto below = [&](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };  // keys before key + n
-          uint32_t m = below(min(pos + 1, r.kv_end) - key);
-          if (p.window > 0) m &= ~below(pos - p.window + 1 - key) | below(p.sinks - key);
-          return m;
-        };
+        if (!open) {
+          // a tile that some row sees in part: hidden scores become -inf first, so that the
+          // loops below stay short (the roles' loops have to fit the instruction caches
+          // together: unrolling V's conversion by four cost 15 % of the kernel)
+          auto below = [&](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };  // keys before a tile's n-th
+#pragma unroll 1
+          for (int c = 0; c < kTile / 16; ++c) {
+            const int key = key0 + 16 * c;
+            uint32_t m = below(min(pos + 1, r.kv_end) - key);
+            if (p.window > 0) m &= ~below(pos - p.window + 1 - key) | below(p.sinks - key);
+            float y[16];
+            tc::ld_wait(t_s + 16 * c, y);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) y[k] = m >> k & 1 ? y[k] : -INFINITY;
+            tc::st(t_s + 16 * c, y);
+          }
+          tc::wait_st();
+        }
         const float4* sc = S.scale[i % kScales];  // written before K's stage was full
         // the tile's maximum (loops kept short: the softmax warps' code has to stay in the
         // instruction caches beside the other roles')
@@ -643,11 +662,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 2; ++c) {
           float s[32];
           tc::ld32_wait(t_s + 32 * c, s);
-          if (!open) {
-            const uint32_t m = visible(key0 + 32 * c);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) s[k] = m >> k & 1 ? s[k] : -INFINITY;
-          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float* y = s + 16 * h;
@@ -683,11 +697,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 2; ++c) {
           float s[32], pk[16];
           tc::ld32_wait(t_s + 32 * c, s);
-          if (!open) {
-            const uint32_t m = visible(key0 + 32 * c);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) s[k] = m >> k & 1 ? s[k] : -INFINITY;
-          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float4 f = sc[(32 * c + 16 * h) >> p.shift];
@@ -724,34 +733,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_after_sync();
       const float f = whole ? (l > 0.f ? __fdividef(256.f, l) : 0.f) : 256.f;  // V entered as 2^-8 V
       __nv_bfloat16* dst =
-          p.out + (int64_t)(r.row0 + (valid ? t : 0)) * p.o_st + (int64_t)(kh * p.group + row % p.group) * p.o_sh;
+          p.out + (int64_t)(r.row0 + (valid ? t : 0)) * p.o_st + (int64_t)(kh * p.group + row - tok * p.group) * p.o_sh;
       float* pdst = part + (X * kRows + row) * kHead;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float o[32];
+      for (int c = 0; c < 8; ++c) {
+        float o[16];
         if (!first) {
-          tc::ld32_wait(t_o + 32 * c, o);
+          tc::ld_wait(t_o + 16 * c, o);
         } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0.f;
+          for (int k = 0; k < 16; ++k) o[k] = 0.f;
         }
 #pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] *= f;
+        for (int k = 0; k < 16; ++k) o[k] *= f;
         if (valid && whole) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
+          for (int k = 0; k < 16; k += 8) {
             uint32_t u[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const __nv_bfloat162 b = __floats2bfloat162_rn(o[k + 2 * e], o[k + 2 * e + 1]);
               u[e] = *reinterpret_cast<const uint32_t*>(&b);
             }
-            *reinterpret_cast<uint4*>(dst + 32 * c + k) = make_uint4(u[0], u[1], u[2], u[3]);
+            *reinterpret_cast<uint4*>(dst + 16 * c + k) = make_uint4(u[0], u[1], u[2], u[3]);
           }
         } else if (valid) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 4)
-            *reinterpret_cast<float4*>(pdst + 32 * c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          for (int k = 0; k < 16; k += 4)
+            *reinterpret_cast<float4*>(pdst + 16 * c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
       }
       if (!whole && valid)
