@@ -173,7 +173,9 @@ lib.b200kv_block_attn.restype = _i32
 lib.b200kv_block_attn.argtypes = [ctypes.c_char_p, ctypes.c_char_p, _vp]
 lib.b200kv_spec_verify.restype = _i32
 lib.b200kv_spec_verify.argtypes = [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _i32,
-                                   _i32, _vp]
+                                   _i32, _vp, ctypes.c_size_t, _vp]
+lib.b200kv_spec_verify_workspace_bytes.restype = ctypes.c_size_t
+lib.b200kv_spec_verify_workspace_bytes.argtypes = [_i32, _i32, _i32]
 
 KV_FP8_E4M3 = 0
 KV_BF16 = 1

@@ -130,7 +130,8 @@ int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args*
 int spec_verify_launch(const void* logits, int64_t ld, int half, const int64_t* tokens, const int32_t* cu,
                        const float* uniforms, const float* noise, int64_t noise_ld, const float* temperature,
                        const float* draft, int64_t draft_ld, int64_t* out, int32_t* accepted, int num_seqs,
-                       int num_rows, int vocab, void* stream);
+                       int num_rows, int vocab, void* workspace, size_t workspace_bytes, void* stream);
+size_t spec_verify_workspace_bytes(int num_seqs, int num_rows, int vocab);
 
 void set_last_error(int e) { t_last_error = e; }
 
@@ -365,10 +366,14 @@ extern "C" int b200kv_spec_verify(const void* logits, int64_t ld, int half, cons
                                   const int32_t* cu_rows, const float* uniforms, const float* noise,
                                   int64_t noise_ld, const float* temperature, const float* draft_probs,
                                   int64_t draft_ld, int64_t* out_tokens, int32_t* num_accepted, int num_seqs,
-                                  int num_rows, int vocab, void* stream) {
+                                  int num_rows, int vocab, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
   return b200kv::spec_verify_launch(logits, ld, half, tokens, cu_rows, uniforms, noise, noise_ld, temperature,
                                     draft_probs, draft_ld, out_tokens, num_accepted, num_seqs, num_rows, vocab,
-                                    stream);
+                                    workspace, workspace_bytes, stream);
+}
+extern "C" size_t b200kv_spec_verify_workspace_bytes(int num_seqs, int num_rows, int vocab) {
+  return b200kv::spec_verify_workspace_bytes(num_seqs, num_rows, vocab);
 }
 
 // ---- tensor-parallel allreduce over peer memory ------------------------------------

@@ -5,14 +5,19 @@
 // (p after the last draft) and e ~ Exp(1): the race that v wins with probability
 // w(v) / sum w, with no prefix sum over the vocabulary.
 //
-// One cluster of kCs CTAs per sequence, a contiguous chunk of the vocabulary each.
-// Per row every CTA reduces its chunk to (max, sum of exponentials, lowest index of
-// the maximum) with an online softmax per thread; the ranks read each other's
-// through distributed shared memory, so every CTA knows which row stops, and races
-// its chunk of that row.  Statistics are fp32, the temperature divides as a
-// multiplication by its reciprocal.
+// Two launches over (row, chunk of the vocabulary) and (sequence, chunk):
+//  * statistics: a row's chunk to (max, sum of exponentials), for a greedy sequence
+//    (max, its lowest index), online over 16 elements of a thread at a time;
+//  * race: every CTA joins its sequence's statistics, finds the row that stops, and
+//    races its chunk of that row; the last CTA of the sequence to arrive (a counter
+//    that the first launch zeroes) picks the winner and writes the tokens.
+// One cluster of 8 or 16 CTAs a sequence in a single launch, joined through distributed
+// shared memory, measured 19 us for one sequence and 243 us for 64 (few clusters are
+// resident at once, and their barriers leave the memory idle).
+//
+// Statistics are fp32; the temperature divides as a multiplication by its
+// reciprocal.  Streaming the logits bounds a full batch (320 rows of 128256: 164 MB).
 
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <float.h>
@@ -21,14 +26,16 @@
 #include "b200kv.h"
 #include "b200kv_common.cuh"
 
-namespace cg = cooperative_groups;
-
 namespace b200kv {
 namespace {
 
-constexpr int kCs = 8;
-constexpr int kThr = 512;
-constexpr int kBatch = 8;  // rows whose statistics are exchanged together
+constexpr int kThr = 256;
+constexpr int kRun = 16;      // elements of a thread in flight: logits
+constexpr int kRaceRun = 8;   // and of each of the race's three streams
+constexpr int kMaxChunks = 64;
+constexpr int kMinChunk = 2048;
+constexpr int kBatch = 32;    // rows of a sequence joined together
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct VerifyParams {
   const void* logits;
@@ -43,9 +50,15 @@ struct VerifyParams {
   int64_t draft_ld;
   int64_t* out;
   int32_t* accepted;
-  int vocab;
+  int vocab, num_seqs;
+  int chunk, chunks;    // of the statistics
+  int rchunk, rchunks;  // of the races
+  float4* stats;   // [rows][chunks]: max, sum, lowest index
+  float4* races;   // [num_seqs][rchunks]: residual / noise, its index, p / noise, its index
+  int* counters;   // [num_seqs]
 };
 
+// the sum of exp((x - m) / T), or for greedy rows the lowest index of m
 struct Stat {
   float m, z;
   int best;
@@ -56,175 +69,354 @@ __device__ __forceinline__ float clean(float x) { return x == x ? fminf(x, FLT_M
 template <bool HALF>
 __device__ __forceinline__ float logit(const void* row, int i) {
   if constexpr (HALF) return clean(__bfloat162float(static_cast<const __nv_bfloat16*>(row)[i]));
-  else return clean(static_cast<const float*>(row)[i]);
+  else return clean(__ldg(static_cast<const float*>(row) + i));
 }
-// (m, z): the sum of exp((x - m) / T); -inf is the empty sum
-__device__ __forceinline__ Stat join(Stat a, Stat b, float inv_t) {
-  if (b.m > a.m || (b.m == a.m && b.best < a.best)) {
-    const Stat t = a;
-    a = b;
-    b = t;
+// A thread's elements of a run of RUN * kThr from `base`: with VEC four adjacent ones at
+// a time, element k at base + at<VEC>(k).
+template <bool VEC>
+__device__ __forceinline__ int at(int k) {
+  return VEC ? 4 * (int)threadIdx.x + (k & 3) + (k >> 2) * 4 * kThr : (int)threadIdx.x + k * kThr;
+}
+// x[k] = row[base + at(k)], `none` from hi on.  All loads are issued before any is used.
+template <bool HALF, bool VEC, int RUN>
+__device__ __forceinline__ void load_run(float (&x)[RUN], const void* row, int base, int hi, float none) {
+  if (VEC && base + RUN * kThr <= hi) {
+    if constexpr (HALF) {
+      uint2 v[RUN / 4];
+#pragma unroll
+      for (int k = 0; k < RUN / 4; ++k)
+        v[k] = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(row) + base + at<true>(4 * k)));
+#pragma unroll
+      for (int k = 0; k < RUN; ++k) {
+        const uint32_t w = k & 2 ? v[k / 4].y : v[k / 4].x;
+        x[k] = __uint_as_float(k & 1 ? w & 0xFFFF0000u : w << 16);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < RUN; k += 4)
+        *reinterpret_cast<float4*>(x + k) =
+            __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(row) + base + at<true>(k)));
+    }
+    return;
   }
-  if (b.m != -INFINITY) a.z += b.z * __expf((b.m - a.m) * inv_t);
-  return a;
+#pragma unroll
+  for (int k = 0; k < RUN; ++k) {
+    const int j = base + at<VEC>(k);
+    x[k] = none;
+    if (j < hi) {
+      if constexpr (HALF) x[k] = __bfloat162float(static_cast<const __nv_bfloat16*>(row)[j]);
+      else x[k] = __ldg(static_cast<const float*>(row) + j);
+    }
+  }
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+// The warp's statistic of its lanes', in every lane; c = log2(e) / T.
+__device__ __forceinline__ Stat join_warp(Stat s, float c) {
+  const float m = warp_max(s.m);
+  float z = m == -INFINITY ? 0.f : s.z * ex2((s.m - m) * c);  // ex2(-inf) = 0
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+  const int best = __reduce_min_sync(0xffffffffu, s.m == m ? s.best : INT32_MAX);
+  return {m, z, best};
 }
 
 struct Race {
   float w;   // residual / noise
   int i;
-  float wp;  // p / noise
+  float wp;  // p / noise, should no residual be left
   int ip;
 };
 __device__ __forceinline__ Race win(Race a, const Race& b) {
-  if (b.w > a.w || (b.w == a.w && b.i < a.i)) { a.w = b.w; a.i = b.i; }
-  if (b.wp > a.wp || (b.wp == a.wp && b.ip < a.ip)) { a.wp = b.wp; a.ip = b.ip; }
+  if (b.w > a.w || (b.w == a.w && b.i < a.i)) {
+    a.w = b.w;
+    a.i = b.i;
+  }
+  if (b.wp > a.wp || (b.wp == a.wp && b.ip < a.ip)) {
+    a.wp = b.wp;
+    a.ip = b.ip;
+  }
   return a;
+}
+__device__ __forceinline__ Race win_warp(Race r) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Race t;
+    t.w = __shfl_xor_sync(0xffffffffu, r.w, o);
+    t.i = __shfl_xor_sync(0xffffffffu, r.i, o);
+    t.wp = __shfl_xor_sync(0xffffffffu, r.wp, o);
+    t.ip = __shfl_xor_sync(0xffffffffu, r.ip, o);
+    r = win(r, t);
+  }
+  return r;
 }
 
 template <bool HALF>
-__global__ void __cluster_dims__(kCs, 1, 1) __launch_bounds__(kThr) spec_verify_kernel(const VerifyParams p) {
-  __shared__ Stat s_warp[kThr / 32][kBatch];
-  __shared__ Stat s_mine[kBatch];
-  __shared__ Race s_race[kThr / 32];
-  __shared__ Race s_won;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), seq = blockIdx.y;
+__device__ __forceinline__ const void* row_of(const VerifyParams& p, int r) {
+  return static_cast<const char*>(p.logits) + (int64_t)r * p.ld * (HALF ? 2 : 4);
+}
+// log2(e) / T; T <= 0 is greedy
+__device__ __forceinline__ float factor(const VerifyParams& p, int seq, bool& greedy) {
+  const float t = p.temperature ? p.temperature[seq] : 1.f;
+  greedy = !(t > 0.f);
+  return greedy ? kLog2e : __fdiv_rn(1.f, t) * kLog2e;
+}
+
+template <bool HALF, bool VEC>
+__global__ void __launch_bounds__(kThr) spec_stats_kernel(const VerifyParams p) {
+  __shared__ Stat s_warp[kThr / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r = blockIdx.x / p.chunks, ch = blockIdx.x - r * p.chunks;
+  if (tid == 0) griddep_launch_dependents();
+  griddep_wait();
+  for (int i = blockIdx.x * kThr + tid; i < p.num_seqs; i += gridDim.x * kThr) p.counters[i] = 0;
+  const void* row = row_of<HALF>(p, r);
+  const int lo = ch * p.chunk, hi = min(p.vocab, lo + p.chunk);
+  float x[kRun];
+  load_run<HALF, VEC>(x, row, lo, hi, -INFINITY);
+  int seq = 0;  // of row r: the sequences that end before it
+  for (int i = 0; i < p.num_seqs; i += kThr)
+    seq += __syncthreads_count(i + tid < p.num_seqs && p.cu[min(i + tid, p.num_seqs - 1) + 1] <= r);
+  if (seq >= p.num_seqs) return;  // a row of nobody
+  bool greedy;
+  const float c = factor(p, seq, greedy);
+  Stat st = {-INFINITY, 0.f, INT32_MAX};
+  for (int base = lo;;) {
+    float m = st.m;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      x[k] = clean(x[k]);
+      m = fmaxf(m, x[k]);
+    }
+    if (greedy) {
+      if (m > st.m) {
+#pragma unroll
+        for (int k = kRun - 1; k >= 0; --k)
+          if (x[k] == m) st.best = base + at<VEC>(k);
+      }
+    } else if (m != -INFINITY) {
+      float z = st.z * ex2((st.m - m) * c);
+#pragma unroll
+      for (int k = 0; k < kRun; ++k) z += ex2((x[k] - m) * c);
+      st.z = z;
+    }
+    st.m = m;
+    base += kRun * kThr;
+    if (base >= hi) break;
+    load_run<HALF, VEC>(x, row, base, hi, -INFINITY);
+  }
+  st = join_warp(st, c);
+  if (lane == 0) s_warp[warp] = st;
+  __syncthreads();
+  if (warp == 0) {
+    st = join_warp(lane < kThr / 32 ? s_warp[lane] : Stat{-INFINITY, 0.f, INT32_MAX}, c);
+    if (lane == 0) p.stats[blockIdx.x] = make_float4(st.m, st.z, __int_as_float(st.best), 0.f);
+  }
+}
+
+template <bool HALF, bool VEC>
+__global__ void __launch_bounds__(kThr) spec_race_kernel(const VerifyParams p) {
+  __shared__ Stat s_row[kBatch];
+  __shared__ float s_x[kBatch], s_q[kBatch], s_u[kBatch];  // of each row's draft
+  __shared__ Race s_race[kThr / 32];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int seq = blockIdx.x / p.rchunks, ch = blockIdx.x - seq * p.rchunks;
   if (tid == 0) griddep_launch_dependents();
   griddep_wait();
   const int r0 = p.cu[seq], n = p.cu[seq + 1] - r0;
-  if (n <= 0) {  // no rows: nothing to verify (the whole cluster leaves)
-    if (rank == 0 && tid == 0) p.accepted[seq] = 0;
+  if (n <= 0) {  // no rows: nothing to verify
+    if (ch == 0 && tid == 0) p.accepted[seq] = 0;
     return;
   }
-  const float temp = p.temperature ? p.temperature[seq] : 1.f;
-  const bool greedy = !(temp > 0.f);
-  const float inv_t = greedy ? 1.f : __fdiv_rn(1.f, temp);
-  const int chunk = (p.vocab + kCs - 1) / kCs;
-  const int lo = min(p.vocab, rank * chunk), hi = min(p.vocab, lo + chunk);
-  const int esz = HALF ? 2 : 4;
-  auto row_of = [&](int i) { return static_cast<const char*>(p.logits) + (int64_t)(r0 + i) * p.ld * esz; };
+  bool greedy;
+  const float c = factor(p, seq, greedy);
 
   int stop = n - 1;
-  Stat at = {-INFINITY, 0.f, 0};
+  Stat top = {-INFINITY, 0.f, 0};
   for (int b0 = 0; b0 < n; b0 += kBatch) {
     const int nb = min(kBatch, n - b0);
-    for (int b = 0; b < nb; ++b) {
-      const char* row = row_of(b0 + b);
-      Stat st = {-INFINITY, 0.f, INT32_MAX};
-      for (int i = lo + tid; i < hi; i += kThr) {
-        const float x = logit<HALF>(row, i);
-        if (x > st.m) {
-          st.z = st.z * __expf((st.m - x) * inv_t) + 1.f;  // exp(-inf) = 0 at the first
-          st.m = x;
-          st.best = i;
-        } else if (x != -INFINITY) {
-          st.z += __expf((x - st.m) * inv_t);
+    if (tid < nb && b0 + tid + 1 < n) {
+      const int r = r0 + b0 + tid;
+      const int64_t d = p.tokens[r + 1];
+      const bool ok = d >= 0 && d < p.vocab;  // a draft outside the vocabulary is not taken: q = inf
+      s_x[tid] = ok ? logit<HALF>(row_of<HALF>(p, r), (int)d) : -INFINITY;
+      s_q[tid] = !ok ? INFINITY : p.draft ? p.draft[(int64_t)r * p.draft_ld + d] : 1.f;
+      s_u[tid] = p.uniforms[r];
+    }
+    for (int b = warp; b < nb; b += kThr / 32) {
+      const float4* s = p.stats + (int64_t)(r0 + b0 + b) * p.chunks;
+      Stat st[kMaxChunks / 32];
+#pragma unroll
+      for (int k = 0; k < kMaxChunks / 32; ++k) {
+        st[k] = {-INFINITY, 0.f, INT32_MAX};
+        if (lane + 32 * k < p.chunks) {
+          const float4 v = __ldcg(s + lane + 32 * k);
+          st[k] = {v.x, v.y, __float_as_int(v.z)};
         }
       }
+      const float m = warp_max(fmaxf(st[0].m, st[1].m));
+      float z = 0.f;
+      int best = INT32_MAX;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        Stat ot;
-        ot.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-        ot.z = __shfl_xor_sync(0xffffffffu, st.z, o);
-        ot.best = __shfl_xor_sync(0xffffffffu, st.best, o);
-        st = join(st, ot, inv_t);
+      for (int k = 0; k < kMaxChunks / 32; ++k) {
+        if (m != -INFINITY) z = fmaf(st[k].z, ex2((st[k].m - m) * c), z);
+        if (st[k].m == m) best = min(best, st[k].best);
       }
-      if (lane == 0) s_warp[warp][b] = st;
+      const Stat all = join_warp({m, z, best}, c);
+      if (lane == 0) s_row[b] = {all.m, all.z, all.best == INT32_MAX ? 0 : all.best};
     }
     __syncthreads();
-    if (tid < nb) {
-      Stat st = s_warp[0][tid];
-      for (int w = 1; w < kThr / 32; ++w) st = join(st, s_warp[w][tid], inv_t);
-      s_mine[tid] = st;
-    }
-    cluster.sync();
     bool done = false;
-    for (int b = 0; b < nb && !done; ++b) {  // every thread of every rank finds the same answer
-      Stat st = {-INFINITY, 0.f, INT32_MAX};
-      for (int r = 0; r < kCs; ++r) st = join(st, *cluster.map_shared_rank(&s_mine[b], r), inv_t);
-      if (st.best == INT32_MAX) st.best = 0;
-      at = st;
+    for (int b = 0; b < nb && !done; ++b) {  // every thread of the sequence's CTAs finds the same answer
+      top = s_row[b];
       stop = b0 + b;
       if (stop == n - 1) break;
-      const int64_t d = p.tokens[r0 + stop + 1];
-      bool take = false;
-      if (d >= 0 && d < p.vocab) {
-        const float x = logit<HALF>(row_of(stop), (int)d);
-        const float pd = greedy ? (d == st.best && st.m != -INFINITY ? 1.f : 0.f)
-                                : (x == -INFINITY ? 0.f : __expf((x - st.m) * inv_t) / st.z);
-        const float qd = p.draft ? p.draft[(int64_t)(r0 + stop) * p.draft_ld + d] : 1.f;
-        take = p.uniforms[r0 + stop] * qd < pd;
-      }
-      done = !take;
+      const float pd = top.m == -INFINITY ? 0.f
+                       : greedy          ? (p.tokens[r0 + stop + 1] == top.best ? 1.f : 0.f)
+                                         : __fdividef(ex2((s_x[b] - top.m) * c), top.z);
+      done = !(s_u[b] * s_q[b] < pd);
     }
-    cluster.sync();  // the ranks have read each other's statistics
     if (done) break;
+    __syncthreads();  // the rows' values are written again
   }
 
-  // ---- the race over row `stop` ------------------------------------------------------
   const bool last = stop == n - 1;
-  int token = at.best;
-  if (!greedy && at.m != -INFINITY) {  // a greedy row, or one of -inf, emits its argmax
+  int token = top.best;
+  if (!greedy && top.m != -INFINITY) {  // a greedy row, or one of -inf, emits its argmax
     const int64_t d = last ? -1 : p.tokens[r0 + stop + 1];
+    const int one = !last && !p.draft && d >= 0 && d < p.vocab ? (int)d : -1;  // where an undrawn draft's q is
     const float* q = !last && p.draft ? p.draft + (int64_t)(r0 + stop) * p.draft_ld : nullptr;
     const float* e = p.noise + (int64_t)seq * p.noise_ld;
-    const char* row = row_of(stop);
-    const float inv_z = 1.f / at.z;
+    const void* row = row_of<HALF>(p, r0 + stop);
+    const float inv_z = __fdividef(1.f, top.z);
+    const int lo = ch * p.rchunk, hi = min(p.vocab, lo + p.rchunk);
     Race rc = {-1.f, INT32_MAX, -1.f, INT32_MAX};
-    for (int i = lo + tid; i < hi; i += kThr) {
-      const float x = logit<HALF>(row, i);
-      const float pv = x == -INFINITY ? 0.f : __expf((x - at.m) * inv_t) * inv_z;
-      const float qv = q ? q[i] : (i == d ? 1.f : 0.f);
-      const float ie = 1.f / fmaxf(e[i], FLT_MIN);
-      const float w = fmaxf(pv - qv, 0.f) * ie, wp = pv * ie;
-      if (w > rc.w) { rc.w = w; rc.i = i; }
-      if (wp > rc.wp) { rc.wp = wp; rc.ip = i; }
-    }
+    for (int base = lo; base < hi; base += kRaceRun * kThr) {
+      float x[kRaceRun], y[kRaceRun], s[kRaceRun];
+      load_run<HALF, VEC>(x, row, base, hi, -INFINITY);
+      load_run<false, VEC>(y, e, base, hi, 1.f);
+      if (q) {
+        load_run<false, VEC>(s, q, base, hi, 0.f);
+      } else {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      Race ot;
-      ot.w = __shfl_xor_sync(0xffffffffu, rc.w, o);
-      ot.i = __shfl_xor_sync(0xffffffffu, rc.i, o);
-      ot.wp = __shfl_xor_sync(0xffffffffu, rc.wp, o);
-      ot.ip = __shfl_xor_sync(0xffffffffu, rc.ip, o);
-      rc = win(rc, ot);
+        for (int k = 0; k < kRaceRun; ++k) s[k] = base + at<VEC>(k) == one ? 1.f : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < kRaceRun; ++k) {
+        const int j = base + at<VEC>(k);
+        const float pv = ex2((clean(x[k]) - top.m) * c) * inv_z, ie = __fdividef(1.f, fmaxf(y[k], FLT_MIN));
+        const float w = j < hi ? fmaxf(pv - s[k], 0.f) * ie : -1.f, wp = j < hi ? pv * ie : -1.f;
+        if (w > rc.w) {
+          rc.w = w;
+          rc.i = j;
+        }
+        if (wp > rc.wp) {
+          rc.wp = wp;
+          rc.ip = j;
+        }
+      }
     }
+    rc = win_warp(rc);
     if (lane == 0) s_race[warp] = rc;
     __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < kThr / 32; ++w) rc = win(rc, s_race[w]);
-      s_won = rc;
+    if (warp == 0) {
+      const Race none = {-1.f, INT32_MAX, -1.f, INT32_MAX};
+      rc = win_warp(lane < kThr / 32 ? s_race[lane] : none);
+      float4* races = p.races + (int64_t)seq * p.rchunks;
+      int arrived = 0;
+      if (lane == 0) {
+        races[ch] = make_float4(rc.w, __int_as_float(rc.i), rc.wp, __int_as_float(rc.ip));
+        __threadfence();
+        arrived = atomicAdd(p.counters + seq, 1);
+        __threadfence();
+      }
+      arrived = __shfl_sync(0xffffffffu, arrived, 0);
+      if (arrived == p.rchunks - 1) {
+        rc = none;
+        for (int k = lane; k < p.rchunks; k += 32) {
+          const float4 v = __ldcg(races + k);
+          rc = win(rc, {v.x, __float_as_int(v.y), v.z, __float_as_int(v.w)});
+        }
+        rc = win_warp(rc);
+        token = rc.w > 0.f ? rc.i : rc.ip;
+      }
+      if (lane == 0) {
+        s_last = arrived == p.rchunks - 1;
+        s_race[0].i = token;
+      }
     }
-    cluster.sync();
-    if (rank == 0 && tid == 0) {
-      for (int r = 1; r < kCs; ++r) rc = win(rc, *cluster.map_shared_rank(&s_won, r));
-      token = rc.w > 0.f ? rc.i : rc.ip;
-    }
-    cluster.sync();  // peers keep their shared memory until rank 0 has read it
+    __syncthreads();
+    if (!s_last) return;
+    token = s_race[0].i;
+  } else if (ch != 0) {
+    return;
   }
-  if (rank == 0) {
-    for (int i = tid; i < n; i += kThr)
-      if (i != stop) p.out[r0 + i] = i < stop ? p.tokens[r0 + i + 1] : -1;
-    if (tid == 0) {
-      p.out[r0 + stop] = token;
-      p.accepted[seq] = stop;
-    }
-  }
+  for (int i = tid; i < n; i += kThr)
+    p.out[r0 + i] = i < stop ? p.tokens[r0 + i + 1] : (i == stop ? token : -1);
+  if (tid == 0) p.accepted[seq] = stop;
+}
+
+template <bool HALF, bool VEC>
+cudaError_t launch(const VerifyParams& p, int num_rows, cudaStream_t st) {
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)num_rows * p.chunks, 1, 1);
+  lc.blockDim = dim3(kThr, 1, 1);
+  lc.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = attr;
+  lc.numAttrs = pdl_enabled() ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&lc, spec_stats_kernel<HALF, VEC>, p);
+  if (e != cudaSuccess) return e;
+  lc.gridDim = dim3((unsigned)p.num_seqs * p.rchunks, 1, 1);
+  return cudaLaunchKernelEx(&lc, spec_race_kernel<HALF, VEC>, p);
+}
+
+// Elements of a chunk of `rows` rows: the most, of 2048 to 16384,
+// that still give every SM `per_sm` CTAs (8 sequences of 5 rows of 128256 took 68 us
+// with chunks of 16384, 34 with small ones); at most kMaxChunks chunks a row.
+int chunk_of(int rows, int vocab, int per_sm) {
+  int chunk = 16384;
+  const int sms = num_sms_current_device() > 0 ? num_sms_current_device() : 148;
+  while (chunk > kMinChunk && (int64_t)rows * cdiv(vocab, chunk) < (int64_t)per_sm * sms) chunk /= 2;
+  const int least = (cdiv(vocab, kMaxChunks) + kMinChunk - 1) / kMinChunk * kMinChunk;
+  return chunk > least ? chunk : least;
 }
 
 }  // namespace
 
+// statistics and races of the most chunks that the sizes can have, counters
+size_t spec_verify_workspace_bytes(int num_seqs, int num_rows, int vocab) {
+  if (num_seqs < 0 || num_rows < 0 || vocab <= 0) return 0;
+  const int least = (cdiv(vocab, kMaxChunks) + kMinChunk - 1) / kMinChunk * kMinChunk;
+  const size_t chunks = cdiv(vocab, kMinChunk > least ? kMinChunk : least);
+  return ((size_t)num_rows + num_seqs) * chunks * sizeof(float4) + align_up((size_t)num_seqs * sizeof(int), 16);
+}
+
 int spec_verify_launch(const void* logits, int64_t ld, int half, const int64_t* tokens, const int32_t* cu,
                        const float* uniforms, const float* noise, int64_t noise_ld, const float* temperature,
                        const float* draft, int64_t draft_ld, int64_t* out, int32_t* accepted, int num_seqs,
-                       int num_rows, int vocab, void* stream) {
+                       int num_rows, int vocab, void* workspace, size_t workspace_bytes, void* stream) {
   if (!logits || !tokens || !cu || !uniforms || !noise || !out || !accepted) return B200KV_ERR_INVALID_ARG;
   if (num_seqs < 0 || num_rows < 0 || vocab <= 0 || ld < vocab || noise_ld < vocab || (draft && draft_ld < vocab))
     return B200KV_ERR_INVALID_ARG;
-  if (num_seqs > 65535) return B200KV_ERR_UNSUPPORTED;
+  if ((int64_t)num_rows * kMaxChunks > 0x7fffffff || (int64_t)num_seqs * kMaxChunks > 0x7fffffff)
+    return B200KV_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < spec_verify_workspace_bytes(num_seqs, num_rows, vocab))
+    return B200KV_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return B200KV_ERR_MISALIGNED;
   if (sm_major_current_device() < 10) return B200KV_ERR_NO_DEVICE;
-  if (num_seqs == 0) return B200KV_OK;
+  if (num_seqs == 0 || num_rows == 0) return B200KV_OK;
   VerifyParams p;
   p.logits = logits;
   p.ld = ld;
@@ -239,17 +431,24 @@ int spec_verify_launch(const void* logits, int64_t ld, int half, const int64_t* 
   p.out = out;
   p.accepted = accepted;
   p.vocab = vocab;
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(kCs, num_seqs, 1);
-  lc.blockDim = dim3(kThr, 1, 1);
-  lc.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  lc.attrs = attr;
-  lc.numAttrs = pdl_enabled() ? 1 : 0;
-  const cudaError_t e = half ? cudaLaunchKernelEx(&lc, spec_verify_kernel<true>, p)
-                             : cudaLaunchKernelEx(&lc, spec_verify_kernel<false>, p);
+  p.num_seqs = num_seqs;
+  p.chunk = chunk_of(num_rows, vocab, 12);
+  p.chunks = cdiv(vocab, p.chunk);
+  p.stats = static_cast<float4*>(workspace);
+  p.rchunk = chunk_of(num_seqs, vocab, 6);
+  p.rchunks = cdiv(vocab, p.rchunk);
+  p.races = p.stats + (size_t)num_rows * p.chunks;
+  p.counters = reinterpret_cast<int*>(p.races + (size_t)num_seqs * p.rchunks);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // four elements at a time where every row begins on their boundary
+  const uintptr_t wide = reinterpret_cast<uintptr_t>(noise) | reinterpret_cast<uintptr_t>(draft);
+  const bool vec = (ld | noise_ld | draft_ld) % 4 == 0 && wide % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(logits) % (half ? 8 : 16) == 0;
+  cudaError_t e;
+  if (half)
+    e = vec ? launch<true, true>(p, num_rows, st) : launch<true, false>(p, num_rows, st);
+  else
+    e = vec ? launch<false, true>(p, num_rows, st) : launch<false, false>(p, num_rows, st);
   return e == cudaSuccess ? B200KV_OK : B200KV_ERR_LAUNCH;
 }
 

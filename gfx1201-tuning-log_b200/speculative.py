@@ -12,6 +12,8 @@ import torch
 
 from _b200kv import check, lib
 
+_F32, _BF16, _I64, _I32 = torch.float32, torch.bfloat16, torch.int64, torch.int32
+
 
 def verify(logits, tokens, cu_rows, uniforms, noise, temperature=None, draft_probs=None, out_tokens=None,
            num_accepted=None):
@@ -25,44 +27,52 @@ def verify(logits, tokens, cu_rows, uniforms, noise, temperature=None, draft_pro
     such as tokens looked up in the prompt).  Rows cu_rows[s] .. of out_tokens
     hold the sequence's num_accepted[s] taken drafts, the emitted token, then -1.
     """
-    if logits.dtype not in (torch.float32, torch.bfloat16):
+    if logits.dtype is not _F32 and logits.dtype is not _BF16:
         raise TypeError("logits must be float32 or bfloat16")
-    if tokens.dtype != torch.int64 or cu_rows.dtype != torch.int32:
+    if tokens.dtype is not _I64 or cu_rows.dtype is not _I32:
         raise TypeError("tokens must be int64 and cu_rows int32")
-    for name, t in (("uniforms", uniforms), ("noise", noise), ("temperature", temperature),
-                    ("draft_probs", draft_probs)):
-        if t is not None and t.dtype != torch.float32:
-            raise TypeError(f"{name} must be float32")
+    if uniforms.dtype is not _F32 or noise.dtype is not _F32:
+        raise TypeError("uniforms and noise must be float32")
     rows, vocab = logits.shape
     seqs = cu_rows.shape[0] - 1
     if tokens.shape != (rows,) or uniforms.shape != (rows,):
         raise ValueError(f"tokens and uniforms must be [{rows}]")
     if noise.shape != (seqs, vocab):
         raise ValueError(f"noise must be [{seqs}, {vocab}]")
-    if temperature is not None and temperature.shape != (seqs,):
-        raise ValueError(f"temperature must be [{seqs}]")
-    if draft_probs is not None and draft_probs.shape != (rows, vocab):
-        raise ValueError(f"draft_probs must be [{rows}, {vocab}]")
+    ld, one = logits.stride()
+    noise_ld, noise_one = noise.stride()
+    if one != 1 or noise_one != 1:
+        raise ValueError("logits and noise must have unit innermost stride")
+    if not (tokens.is_contiguous() and cu_rows.is_contiguous() and uniforms.is_contiguous()):
+        raise ValueError("tokens, cu_rows and uniforms must be contiguous")
+    heat = draft = draft_ld = 0
+    if temperature is not None:
+        if temperature.dtype is not _F32:
+            raise TypeError("temperature must be float32")
+        if temperature.shape != (seqs,) or not temperature.is_contiguous():
+            raise ValueError(f"temperature must be contiguous [{seqs}]")
+        heat = temperature.data_ptr()
+    if draft_probs is not None:
+        if draft_probs.dtype is not _F32:
+            raise TypeError("draft_probs must be float32")
+        draft_ld, one = draft_probs.stride()
+        if draft_probs.shape != (rows, vocab) or one != 1:
+            raise ValueError(f"draft_probs must be [{rows}, {vocab}] with unit innermost stride")
+        draft = draft_probs.data_ptr()
     if out_tokens is None:
         out_tokens = torch.empty_like(tokens)
-    elif out_tokens.dtype != torch.int64 or out_tokens.shape != (rows,):
-        raise TypeError(f"out_tokens must be int64 [{rows}]")
+    elif out_tokens.dtype is not _I64 or out_tokens.shape != (rows,) or not out_tokens.is_contiguous():
+        raise TypeError(f"out_tokens must be contiguous int64 [{rows}]")
     if num_accepted is None:
-        num_accepted = torch.empty(seqs, dtype=torch.int32, device=logits.device)
-    elif num_accepted.dtype != torch.int32 or num_accepted.shape != (seqs,):
-        raise TypeError(f"num_accepted must be int32 [{seqs}]")
-    for name, t in (("tokens", tokens), ("cu_rows", cu_rows), ("uniforms", uniforms), ("temperature", temperature),
-                    ("out_tokens", out_tokens), ("num_accepted", num_accepted)):
-        if t is not None and not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-    for name, t in (("logits", logits), ("noise", noise), ("draft_probs", draft_probs)):
-        if t is not None and t.stride(1) != 1:
-            raise ValueError(f"{name} must have unit innermost stride")
-    check(lib.b200kv_spec_verify(
-        logits.data_ptr(), logits.stride(0), 1 if logits.dtype == torch.bfloat16 else 0, tokens.data_ptr(),
-        cu_rows.data_ptr(), uniforms.data_ptr(), noise.data_ptr(), noise.stride(0),
-        temperature.data_ptr() if temperature is not None else None,
-        draft_probs.data_ptr() if draft_probs is not None else None,
-        draft_probs.stride(0) if draft_probs is not None else 0, out_tokens.data_ptr(), num_accepted.data_ptr(), seqs,
-        rows, vocab, torch._C._cuda_getCurrentRawStream(logits.device.index)), "b200kv_spec_verify")
+        num_accepted = torch.empty(seqs, dtype=_I32, device=logits.device)
+    elif num_accepted.dtype is not _I32 or num_accepted.shape != (seqs,) or not num_accepted.is_contiguous():
+        raise TypeError(f"num_accepted must be contiguous int32 [{seqs}]")
+    size = lib.b200kv_spec_verify_workspace_bytes(seqs, rows, vocab)
+    scratch = torch.empty(size, dtype=torch.uint8, device=logits.device)
+    status = lib.b200kv_spec_verify(
+        logits.data_ptr(), ld, logits.dtype is _BF16, tokens.data_ptr(), cu_rows.data_ptr(), uniforms.data_ptr(),
+        noise.data_ptr(), noise_ld, heat, draft, draft_ld, out_tokens.data_ptr(), num_accepted.data_ptr(), seqs, rows,
+        vocab, scratch.data_ptr(), size, torch._C._cuda_getCurrentRawStream(logits.device.index))
+    if status:
+        check(status, "b200kv_spec_verify")
     return out_tokens, num_accepted

@@ -515,11 +515,15 @@ int b200kv_block_attn(const b200kv_block_cache* cache, const b200kv_block_attn_a
  *   num_accepted  int32 [num_seqs]: drafts taken
  * A logit of NaN counts as -inf, infinities as the largest finite value; a row of
  * -inf takes no draft and emits token 0.  A draft outside [0, vocab) is not
- * taken.  temperature NULL: 1.  No counterpart in the reference. */
+ * taken.  temperature NULL: 1.  workspace: b200kv_spec_verify_workspace_bytes
+ * bytes, 16-byte aligned, its contents of no account; calls that share one are
+ * ordered on one stream.  No counterpart in the reference. */
+size_t b200kv_spec_verify_workspace_bytes(int num_seqs, int num_rows, int vocab);
 int b200kv_spec_verify(const void* logits, int64_t ld, int half, const int64_t* tokens, const int32_t* cu_rows,
                        const float* uniforms, const float* noise, int64_t noise_ld, const float* temperature,
                        const float* draft_probs, int64_t draft_ld, int64_t* out_tokens, int32_t* num_accepted,
-                       int num_seqs, int num_rows, int vocab, void* stream);
+                       int num_seqs, int num_rows, int vocab, void* workspace, size_t workspace_bytes,
+                       void* stream);
 
 /* ---- Tensor-parallel allreduce over peer memory ---------------------------------
  *
