@@ -13,6 +13,10 @@
 // 128 tokens, keeps their rotated k and v in registers between the maximum and
 // the codes, and rotates the head's group of q rows of the same tokens, whose
 // angles it then reads once.  No atomics on memory: two runs give the same bytes.
+// Half a warp holds a token (8-byte loads and stores, 128 bytes of a row each), all
+// of a token's rows in flight at once; a block's heads are adjacent CTAs, as their
+// rows are in memory.  Streaming bounds a prompt's call; a few tokens' is a chain of
+// three loads (the sequence, its block, the block's scale) beside the rows.
 
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
@@ -101,123 +105,155 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float r) {
   return out;
 }
 
-// TPW tokens of the block per warp, NW warps; lane l holds elements 2l, 2l+1 and
-// 64+2l, 64+2l+1 of each row: two rotary pairs.
-template <int TPW, int NW>
-__global__ void __launch_bounds__(NW * 32) block_append_kernel(const AppendParams p) {
-  __shared__ int s_count[NW];
+struct Item {
+  int seq, row, qlen, total, page;
+};
+
+// PASSES tokens of the block per half warp, NW warps; lane l of the half holds
+// elements 4l .. 4l+3 and 64+4l .. 64+4l+3 of each row: four rotary pairs.
+template <int PASSES, int NW>
+__global__ void __launch_bounds__(NW * 32, 1024 / (NW * 32)) block_append_kernel(const AppendParams p) {
+  __shared__ Item s_item;
   __shared__ uint32_t s_amax[2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int item = blockIdx.x, kh = blockIdx.y;
+  __shared__ float s_old[2];
+  __shared__ int s_blk;
+  const int tid = threadIdx.x, lane = tid & 15, half = tid >> 4;
+  const int item = blockIdx.x / p.hkv, kh = blockIdx.x - item * p.hkv;
   if (tid == 0) griddep_launch_dependents();
   if (tid < 2) s_amax[tid] = 0;
+  if (tid == 2) s_item.qlen = 0;
   griddep_wait();
-
-  // the sequence of this item: the last one whose first item is not past it
-  const int c0 = p.cu[0];
-  int cnt = 0;
-  for (int s = tid; s < p.num_seqs; s += NW * 32) cnt += first_item(p.cu[s] - c0, s, p.shift) <= item;
-  cnt = __reduce_add_sync(0xffffffffu, cnt);
-  if (lane == 0) s_count[warp] = cnt;
   __syncthreads();
-  int seq = -1;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) seq += s_count[w];
-  const int row_s = p.cu[seq], qlen = p.cu[seq + 1] - row_s, total = p.lens[seq];
-  const int begin = total - qlen;
-  const int page = (begin >> p.shift) + (item - first_item(row_s - c0, seq, p.shift));
-  if (qlen <= 0 || page > ((total - 1) >> p.shift)) return;
-  const int lo = max(begin, page << p.shift), hi = min(total, (page + 1) << p.shift);
-  const int nt = hi - lo, row0 = row_s + (lo - begin);
-  const int kept = lo - (page << p.shift);  // earlier tokens of this block
-
-  int blk = -1;
-  if (page >= 0 && page < p.max_blocks) blk = p.bt[(int64_t)seq * p.bt_stride + page];
-  const bool ok = blk >= 0 && blk < p.num_blocks;
-  if (!ok && tid == 0) atomicExch(&g_device_status, kDevIndexRange);
-  float* ksp = p.ks + (int64_t)(ok ? blk : 0) * p.ks0 + kh * p.ks1;
-  float* vsp = p.vs + (int64_t)(ok ? blk : 0) * p.vs0 + kh * p.vs1;
-  const float old_k = ok ? *ksp : 0.f, old_v = ok ? *vsp : 0.f;
+  // the sequence whose items this one is among
+  const int c0 = p.cu[0];
+  for (int s = tid; s < p.num_seqs; s += NW * 32) {
+    const int row = p.cu[s], end = p.cu[s + 1], total = p.lens[s];
+    const int at = item - first_item(row - c0, s, p.shift);
+    if (at >= 0 && (s + 1 == p.num_seqs || item < first_item(end - c0, s + 1, p.shift))) {
+      const int page = ((total - (end - row)) >> p.shift) + at;
+      s_item = {s, row, page <= ((total - 1) >> p.shift) ? end - row : 0, total, page};
+    }
+  }
+  __syncthreads();
+  const Item it = s_item;
+  if (it.qlen <= 0) return;
+  const int begin = it.total - it.qlen, page0 = it.page << p.shift;
+  const int lo = max(begin, page0), hi = min(it.total, page0 + (1 << p.shift));
+  const int nt = hi - lo, row0 = it.row + (lo - begin);
+  const int kept = lo - page0;  // earlier tokens of this block
+  if (tid == 0) {
+    int blk = -1;
+    if (it.page >= 0 && it.page < p.max_blocks) blk = p.bt[(int64_t)it.seq * p.bt_stride + it.page];
+    if (blk < 0 || blk >= p.num_blocks) {
+      blk = -1;
+      atomicExch(&g_device_status, kDevIndexRange);
+    } else if (kept > 0) {
+      s_old[0] = p.ks[(int64_t)blk * p.ks0 + kh * p.ks1];
+      s_old[1] = p.vs[(int64_t)blk * p.vs0 + kh * p.vs1];
+    }
+    s_blk = blk;
+  }
 
   const int group = p.hq / p.hkv;
-  float kr[TPW][4];
-  uint32_t vr[TPW][2];
+  float kr[PASSES][8];
+  uint2 vr[PASSES][2];
   uint32_t amax_k = 0, amax_v = 0;
 #pragma unroll
-  for (int i = 0; i < TPW; ++i) {
-    const int t = warp + i * NW;
+  for (int i = 0; i < PASSES; ++i) {
+    const int t = half + i * 2 * NW;
     if (t < nt) {
       const __nv_bfloat16* row = p.qkv + (int64_t)(row0 + t) * p.qkv_st;
       const int pos = min(max(lo + t, 0), p.max_pos - 1);
-      const float2 c = *reinterpret_cast<const float2*>(p.cos_sin + (int64_t)pos * kHead + 2 * lane);
-      const float2 s = *reinterpret_cast<const float2*>(p.cos_sin + (int64_t)pos * kHead + 64 + 2 * lane);
-      const uint32_t* kw = reinterpret_cast<const uint32_t*>(row + (int64_t)(p.hq + kh) * kHead);
-      const uint32_t* vw = reinterpret_cast<const uint32_t*>(row + (int64_t)(p.hq + p.hkv + kh) * kHead);
-      const uint32_t k1 = kw[lane], k2 = kw[32 + lane];
-      vr[i][0] = vw[lane];
-      vr[i][1] = vw[32 + lane];
-      for (int h = 0; h < group; ++h) {
-        const uint32_t* qw = reinterpret_cast<const uint32_t*>(row + (int64_t)(kh * group + h) * kHead);
-        const uint32_t x1 = qw[lane], x2 = qw[32 + lane];
-        float a1, a2, b1, b2;
-        rope_pair(bf_lo(x1), bf_lo(x2), c.x, s.x, a1, a2);
-        rope_pair(bf_hi(x1), bf_hi(x2), c.y, s.y, b1, b2);
-        uint32_t* o = reinterpret_cast<uint32_t*>(p.q_out + (int64_t)(row0 + t) * p.q_st +
-                                                  (int64_t)(kh * group + h) * p.q_sh);
-        o[lane] = bf_pack(a1, b1);
-        o[32 + lane] = bf_pack(a2, b2);
+      auto load = [&](int head, uint2& a, uint2& b) {
+        const uint2* w = reinterpret_cast<const uint2*>(row + (int64_t)head * kHead);
+        a = w[lane];
+        b = w[16 + lane];
+      };
+      const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos_sin + (int64_t)pos * kHead) + lane);
+      const float4 s = __ldg(reinterpret_cast<const float4*>(p.cos_sin + (int64_t)pos * kHead) + 16 + lane);
+      uint2 k1, k2;
+      load(p.hq + kh, k1, k2);
+      load(p.hq + p.hkv + kh, vr[i][0], vr[i][1]);
+      // y[0 .. 3] and y[4 .. 7]: the pairs' first and second elements
+      auto rotate = [&](const uint2& a, const uint2& b, float (&y)[8]) {
+        rope_pair(bf_lo(a.x), bf_lo(b.x), c.x, s.x, y[0], y[4]);
+        rope_pair(bf_hi(a.x), bf_hi(b.x), c.y, s.y, y[1], y[5]);
+        rope_pair(bf_lo(a.y), bf_lo(b.y), c.z, s.z, y[2], y[6]);
+        rope_pair(bf_hi(a.y), bf_hi(b.y), c.w, s.w, y[3], y[7]);
+      };
+      constexpr int kAhead = 4;  // q rows in flight
+      for (int h0 = 0; h0 < group; h0 += kAhead) {
+        uint2 a[kAhead], b[kAhead];
+#pragma unroll
+        for (int h = 0; h < kAhead; ++h)
+          if (h0 + h < group) load(kh * group + h0 + h, a[h], b[h]);
+#pragma unroll
+        for (int h = 0; h < kAhead; ++h)
+          if (h0 + h < group) {
+            float y[8];
+            rotate(a[h], b[h], y);
+            uint2* o = reinterpret_cast<uint2*>(p.q_out + (int64_t)(row0 + t) * p.q_st +
+                                                (int64_t)(kh * group + h0 + h) * p.q_sh);
+            o[lane] = make_uint2(bf_pack(y[0], y[1]), bf_pack(y[2], y[3]));
+            o[16 + lane] = make_uint2(bf_pack(y[4], y[5]), bf_pack(y[6], y[7]));
+          }
       }
-      rope_pair(bf_lo(k1), bf_lo(k2), c.x, s.x, kr[i][0], kr[i][2]);
-      rope_pair(bf_hi(k1), bf_hi(k2), c.y, s.y, kr[i][1], kr[i][3]);
+      rotate(k1, k2, kr[i]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) amax_k = max(amax_k, finite_bits(kr[i][e]));
+      for (int e = 0; e < 8; ++e) amax_k = max(amax_k, finite_bits(kr[i][e]));
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        amax_v = max(amax_v, max(finite_bits(bf_lo(vr[i][e])), finite_bits(bf_hi(vr[i][e]))));
+      for (int e = 0; e < 2; ++e) {
+        amax_v = max(amax_v, max(finite_bits(bf_lo(vr[i][e].x)), finite_bits(bf_hi(vr[i][e].x))));
+        amax_v = max(amax_v, max(finite_bits(bf_lo(vr[i][e].y)), finite_bits(bf_hi(vr[i][e].y))));
+      }
     }
   }
-  if (!ok) return;  // CTA-uniform
   amax_k = __reduce_max_sync(0xffffffffu, amax_k);
   amax_v = __reduce_max_sync(0xffffffffu, amax_v);
-  if (lane == 0) {
+  if ((tid & 31) == 0) {
     atomicMax(&s_amax[0], amax_k);
     atomicMax(&s_amax[1], amax_v);
   }
   __syncthreads();
+  const int blk = s_blk;
+  if (blk < 0) return;  // CTA-uniform
   float new_k = scale_for(s_amax[0]), new_v = scale_for(s_amax[1]);
   uint8_t* kb = p.kc + (int64_t)blk * p.sk0 + (int64_t)kh * p.sk2;
   uint8_t* vb = p.vc + (int64_t)blk * p.sv0 + (int64_t)kh * p.sv2;
   if (kept > 0) {
+    const float old_k = s_old[0], old_v = s_old[1];
     new_k = fmaxf(new_k, old_k);
     new_v = fmaxf(new_v, old_v);
     const float rk = __fdiv_rn(old_k, new_k), rv = __fdiv_rn(old_v, new_v);
-    for (int t = warp; t < kept; t += NW) {
+    for (int t = tid >> 5; t < kept; t += NW) {
       if (new_k != old_k) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(kb + (int64_t)t * p.sk1) + lane;
+        uint32_t* w = reinterpret_cast<uint32_t*>(kb + (int64_t)t * p.sk1) + (tid & 31);
         *w = rescale4(*w, rk);
       }
       if (new_v != old_v) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(vb + (int64_t)t * p.sv1) + lane;
+        uint32_t* w = reinterpret_cast<uint32_t*>(vb + (int64_t)t * p.sv1) + (tid & 31);
         *w = rescale4(*w, rv);
       }
     }
   }
   if (tid == 0) {
-    *ksp = new_k;
-    *vsp = new_v;
+    p.ks[(int64_t)blk * p.ks0 + kh * p.ks1] = new_k;
+    p.vs[(int64_t)blk * p.vs0 + kh * p.vs1] = new_v;
   }
   const Divider dk(new_k), dv(new_v);
 #pragma unroll
-  for (int i = 0; i < TPW; ++i) {
-    const int t = warp + i * NW;
+  for (int i = 0; i < PASSES; ++i) {
+    const int t = half + i * 2 * NW;
     if (t < nt) {
-      uint16_t* kw = reinterpret_cast<uint16_t*>(kb + (int64_t)(kept + t) * p.sk1);
-      uint16_t* vw = reinterpret_cast<uint16_t*>(vb + (int64_t)(kept + t) * p.sv1);
-      kw[lane] = (uint16_t)codes2(dk(kr[i][0]), dk(kr[i][1]));
-      kw[32 + lane] = (uint16_t)codes2(dk(kr[i][2]), dk(kr[i][3]));
+      uint32_t* kw = reinterpret_cast<uint32_t*>(kb + (int64_t)(kept + t) * p.sk1);
+      uint32_t* vw = reinterpret_cast<uint32_t*>(vb + (int64_t)(kept + t) * p.sv1);
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        vw[32 * e + lane] = (uint16_t)codes2(dv(bf_lo(vr[i][e])), dv(bf_hi(vr[i][e])));
+      for (int e = 0; e < 2; ++e) {
+        const float* y = kr[i] + 4 * e;
+        kw[16 * e + lane] = codes2(dk(y[0]), dk(y[1])) | codes2(dk(y[2]), dk(y[3])) << 16;
+        vw[16 * e + lane] = codes2(dv(bf_lo(vr[i][e].x)), dv(bf_hi(vr[i][e].x))) |
+                            codes2(dv(bf_lo(vr[i][e].y)), dv(bf_hi(vr[i][e].y))) << 16;
+      }
     }
   }
 }
@@ -281,7 +317,9 @@ int block_append_launch(const b200kv_block_cache* c, const void* qkv, int64_t qk
   p.max_blocks = c->max_blocks;
   const int64_t items = (int64_t)(num_tokens >> p.shift) + 2 * (int64_t)c->num_seqs;
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3((unsigned)(items < num_tokens ? items : num_tokens), c->num_kv_heads, 1);
+  const int64_t ctas = (items < num_tokens ? items : num_tokens) * c->num_kv_heads;
+  if (ctas > 0x7fffffff) return B200KV_ERR_UNSUPPORTED;
+  lc.gridDim = dim3((unsigned)ctas, 1, 1);
   lc.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -290,10 +328,10 @@ int block_append_launch(const b200kv_block_cache* c, const void* qkv, int64_t qk
   lc.numAttrs = pdl_enabled() ? 1 : 0;
   cudaError_t e;
   switch (c->block_size) {
-    case 16: lc.blockDim = dim3(256); e = cudaLaunchKernelEx(&lc, block_append_kernel<2, 8>, p); break;
-    case 32: lc.blockDim = dim3(256); e = cudaLaunchKernelEx(&lc, block_append_kernel<4, 8>, p); break;
-    case 64: lc.blockDim = dim3(512); e = cudaLaunchKernelEx(&lc, block_append_kernel<4, 16>, p); break;
-    default: lc.blockDim = dim3(512); e = cudaLaunchKernelEx(&lc, block_append_kernel<8, 16>, p); break;
+    case 16: lc.blockDim = dim3(256); e = cudaLaunchKernelEx(&lc, block_append_kernel<1, 8>, p); break;
+    case 32: lc.blockDim = dim3(256); e = cudaLaunchKernelEx(&lc, block_append_kernel<2, 8>, p); break;
+    case 64: lc.blockDim = dim3(512); e = cudaLaunchKernelEx(&lc, block_append_kernel<2, 16>, p); break;
+    default: lc.blockDim = dim3(512); e = cudaLaunchKernelEx(&lc, block_append_kernel<4, 16>, p); break;
   }
   return e == cudaSuccess ? B200KV_OK : B200KV_ERR_LAUNCH;
 }
