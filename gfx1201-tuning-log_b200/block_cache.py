@@ -33,6 +33,9 @@ def _describe(k_cache, v_cache, k_scales, v_scales, block_table, cu_seqlens, seq
         raise TypeError("block_table, cu_seqlens and seq_lens must be int32")
     shape = k_cache.shape
     nb, bs, hkv, d = shape
+    if not (k_cache.is_cuda and v_cache.is_cuda and k_scales.is_cuda and v_scales.is_cuda and block_table.is_cuda
+            and cu_seqlens.is_cuda and seq_lens.is_cuda):
+        raise ValueError("the cache, cu_seqlens and seq_lens must be on the GPU")
     if v_cache.shape != shape:
         raise ValueError("k_cache and v_cache shapes differ")
     if k_scales.shape != (nb, hkv) or v_scales.shape != (nb, hkv):
@@ -80,12 +83,14 @@ def append(qkv, cos_sin, k_cache, v_cache, k_scales, v_scales, cu_seqlens, seq_l
     if d != HEAD_DIM or not cos_sin.is_contiguous() or one != 1:
         raise ValueError("cos_sin must be contiguous [max_pos, 128] and qkv rows contiguous")
     if q_out is None:
-        q_out = qkv[:, :hq * HEAD_DIM].unflatten(1, (hq, HEAD_DIM))
+        q_out = qkv.as_strided((tokens, hq, HEAD_DIM), (row, HEAD_DIM, 1))  # one view: 0.9 us against 3.7 for two
     elif q_out.dtype is not _BF16:
         raise TypeError("q_out must be bfloat16")
     q0, q1, q2 = q_out.stride()
     if q_out.shape != (tokens, hq, HEAD_DIM) or q2 != 1:
         raise ValueError(f"q_out must be [{tokens}, {hq}, {HEAD_DIM}] with unit innermost stride")
+    if not (qkv.is_cuda and cos_sin.is_cuda and q_out.is_cuda):
+        raise ValueError("qkv, cos_sin and q_out must be on the GPU")
     status = lib.b200kv_block_append(desc, qkv.data_ptr(), row, cos_sin.data_ptr(), positions, q_out.data_ptr(), q0, q1,
                                      cu_seqlens.data_ptr(), seq_lens.data_ptr(), tokens, hq,
                                      _raw_stream(qkv.device.index))
@@ -128,6 +133,8 @@ def attention(q, k_cache, v_cache, k_scales, v_scales, out, cu_seqlens_q, seq_le
     o0, o1, o2 = out.stride()
     if q2 != 1 or o2 != 1:
         raise ValueError("q and out must have unit innermost stride")
+    if not (q.is_cuda and out.is_cuda):
+        raise ValueError("q and out must be on the GPU")
     if workspace is None:
         workspace = Workspace(q.device, seqs, hkv)
     elif workspace.num_seqs < seqs or workspace.num_kv_heads < hkv:

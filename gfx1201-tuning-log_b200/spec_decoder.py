@@ -1,0 +1,118 @@
+"""The MXFP4 decoder with drafted tokens on a block-scaled fp8 cache.
+
+`SpeculativeDecoder` keeps MXFP4Decoder's weights and layers and replaces its
+cache by one with a scale per block and kv head (block_cache), which prompts of
+ragged lengths and verification steps of a few tokens a sequence append to and
+attend over; logits of the drafted tokens go through speculative.verify.  A
+sliding window with first tokens that stay visible (sinks) is an option of the
+whole model.
+
+A step verifies the same number of drafts for every sequence, advances
+positions and last tokens on the device and never waits for it, so it can be
+captured in a CUDA graph.  Rejected drafts stay in the cache past the new
+position and are overwritten by the next step's tokens.
+"""
+import torch
+
+import block_cache
+import decoder
+import speculative
+from _b200kv import check, lib
+
+
+class SpeculativeDecoder(decoder.MXFP4Decoder):
+    """MXFP4Decoder's arguments (one GPU), and window / sinks: a query at
+    position p sees keys j > p - window or j < sinks (window 0: all)."""
+
+    def __init__(self, cfg, device, batch, max_ctx, window=0, sinks=0, **kw):
+        if kw.get("tp", 1) != 1:
+            raise ValueError("SpeculativeDecoder runs on one GPU: a verification reads whole rows of logits")
+        super().__init__(cfg, device, batch, max_ctx, **kw)
+        self.window, self.sinks = window, sinks
+        blocks = self.block_table.numel()
+        for kv in self.kv:
+            kv["ks"] = torch.zeros(blocks, self.hkv, dtype=torch.float32, device=device)
+            kv["vs"] = torch.zeros(blocks, self.hkv, dtype=torch.float32, device=device)
+        self.attn_workspace = block_cache.Workspace(device, batch, self.hkv)
+
+    def forward(self, tokens, cu_seqlens, seq_lens, max_new):
+        """Run new tokens (device int64 [T], sequence s's rows cu_seqlens[s] ..,
+        its length with them seq_lens[s], both device int32) through the layers,
+        appending to the cache; max_new bounds a sequence's rows.  Returns the
+        final hidden rows (bf16 [T, hidden], normalised)."""
+        cfg, d, T = self.cfg, self.cfg.head_dim, tokens.shape[0]
+        new = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device=self.dev)  # noqa: E731
+        h = torch.index_select(self.embed, 0, tokens)
+        x, o, dn = new(T, cfg.hidden), new(T, cfg.hidden), new(T, cfg.hidden)
+        qkv, attn = new(T, (self.hq + 2 * self.hkv) * d), new(T, self.hq, d)
+        gu, act = new(T, 2 * cfg.inter), new(T, cfg.inter)
+        stream = torch.cuda.current_stream(h.device).cuda_stream
+
+        def norm(delta, w):
+            check(lib.b200kv_rmsnorm_residual(h.data_ptr(), delta.data_ptr() if delta is not None else None,
+                                              w.data_ptr(), x.data_ptr(), T, cfg.hidden, float(cfg.eps), stream),
+                  "b200kv_rmsnorm_residual")
+
+        norm(None, self.layers[0]["in_norm"] if self.layers else self.final_norm)
+        for li, lay in enumerate(self.layers):
+            kv = self.kv[li]
+            cache = (kv["k"], kv["v"], kv["ks"], kv["vs"])
+            decoder._gemm(x, lay["qkv"], qkv)
+            q = block_cache.append(qkv, self.rope, *cache, cu_seqlens, seq_lens, self.block_table)
+            block_cache.attention(q, *cache, attn, cu_seqlens, seq_lens, self.block_table, d ** -0.5, max_new,
+                                  max_seq_len=self.max_ctx, window=self.window, sinks=self.sinks,
+                                  workspace=self.attn_workspace)
+            decoder._gemm(attn.view(T, self.hq * d), lay["o"], o)
+            norm(o, lay["post_norm"])
+            decoder._gate_up(x, lay["gate_up"], gu, act, cfg.inter, stream)
+            decoder._gemm(act, lay["down"], dn)
+            norm(dn, self.layers[li + 1]["in_norm"] if li + 1 < len(self.layers) else self.final_norm)
+        return x
+
+    def _logits(self, x):
+        return torch.mm(x, self.lm_head.t(), out_dtype=torch.float32)
+
+    def _sample(self, logits, tokens, cu_rows, temperature, draft_probs, generator):
+        uniforms = torch.rand(logits.shape[0], device=self.dev, generator=generator)
+        noise = torch.empty(self.B, logits.shape[1], device=self.dev).exponential_(generator=generator)
+        return speculative.verify(logits, tokens, cu_rows, uniforms, noise.clamp_min_(1e-30), temperature=temperature,
+                                  draft_probs=draft_probs)
+
+    def prompt(self, prompts, temperature=None, generator=None):
+        """Fill the cache with one prompt a sequence (a list of `batch` int64
+        tensors of any lengths below max_ctx) and draw each one's next token,
+        which is returned and kept in self.tokens; self.positions holds the
+        prompts' lengths.  temperature: float32 [batch] on the device (0 greedy;
+        None: 1)."""
+        if len(prompts) != self.B or not all(0 < len(t) < self.max_ctx for t in prompts):
+            raise ValueError(f"{self.B} prompts of 1 to {self.max_ctx - 1} tokens")
+        lens = torch.tensor([len(t) for t in prompts], dtype=torch.int32)
+        cu = torch.zeros(self.B + 1, dtype=torch.int32)
+        cu[1:] = lens.cumsum(0)
+        cu, dev_lens = cu.to(self.dev), lens.to(self.dev)
+        x = self.forward(torch.cat([t.to(self.dev) for t in prompts]), cu, dev_lens, int(lens.max()))
+        last = self._logits(x[cu[1:].long() - 1])
+        rows = torch.arange(self.B + 1, dtype=torch.int32, device=self.dev)
+        token, _ = self._sample(last, self.tokens, rows, temperature, None, generator)
+        self.tokens.copy_(token)
+        self.positions.copy_(dev_lens)
+        return self.tokens
+
+    def verify_step(self, drafts, temperature=None, draft_probs=None, generator=None):
+        """One step: the last tokens and drafts (int64 [batch, K], K >= 0) through
+        the model, the drafts verified.  Returns (tokens int64 [batch, K + 1], a
+        row's accepted drafts, then the emitted token, then -1; accepted int32
+        [batch]).  draft_probs: float32 [batch, K + 1, vocab], row i the
+        distribution draft i was drawn from (row K is not read; None: drafts that
+        were not drawn).  Positions and last tokens advance in place."""
+        K = drafts.shape[1]
+        fed = torch.cat([self.tokens[:, None], drafts], 1).reshape(-1)
+        cu = torch.arange(0, self.B * (K + 1) + 1, K + 1, dtype=torch.int32, device=self.dev)
+        x = self.forward(fed, cu, self.positions + (K + 1), K + 1)
+        if draft_probs is not None:
+            draft_probs = draft_probs.reshape(self.B * (K + 1), -1)
+        out, accepted = self._sample(self._logits(x), fed, cu, temperature, draft_probs, generator)
+        out = out.view(self.B, K + 1)
+        self.tokens.copy_(out.gather(1, accepted[:, None].long())[:, 0])
+        self.positions.add_(accepted + 1)
+        return out, accepted

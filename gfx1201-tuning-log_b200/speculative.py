@@ -45,19 +45,21 @@ def verify(logits, tokens, cu_rows, uniforms, noise, temperature=None, draft_pro
         raise ValueError("logits and noise must have unit innermost stride")
     if not (tokens.is_contiguous() and cu_rows.is_contiguous() and uniforms.is_contiguous()):
         raise ValueError("tokens, cu_rows and uniforms must be contiguous")
+    if not (logits.is_cuda and tokens.is_cuda and cu_rows.is_cuda and uniforms.is_cuda and noise.is_cuda):
+        raise ValueError("logits, tokens, cu_rows, uniforms and noise must be on the GPU")
     heat = draft = draft_ld = 0
     if temperature is not None:
         if temperature.dtype is not _F32:
             raise TypeError("temperature must be float32")
-        if temperature.shape != (seqs,) or not temperature.is_contiguous():
-            raise ValueError(f"temperature must be contiguous [{seqs}]")
+        if temperature.shape != (seqs,) or not (temperature.is_contiguous() and temperature.is_cuda):
+            raise ValueError(f"temperature must be contiguous [{seqs}] on the GPU")
         heat = temperature.data_ptr()
     if draft_probs is not None:
         if draft_probs.dtype is not _F32:
             raise TypeError("draft_probs must be float32")
         draft_ld, one = draft_probs.stride()
-        if draft_probs.shape != (rows, vocab) or one != 1:
-            raise ValueError(f"draft_probs must be [{rows}, {vocab}] with unit innermost stride")
+        if draft_probs.shape != (rows, vocab) or one != 1 or not draft_probs.is_cuda:
+            raise ValueError(f"draft_probs must be [{rows}, {vocab}] with unit innermost stride, on the GPU")
         draft = draft_probs.data_ptr()
     if out_tokens is None:
         out_tokens = torch.empty_like(tokens)
@@ -67,6 +69,8 @@ def verify(logits, tokens, cu_rows, uniforms, noise, temperature=None, draft_pro
         num_accepted = torch.empty(seqs, dtype=_I32, device=logits.device)
     elif num_accepted.dtype is not _I32 or num_accepted.shape != (seqs,) or not num_accepted.is_contiguous():
         raise TypeError(f"num_accepted must be contiguous int32 [{seqs}]")
+    if not (out_tokens.is_cuda and num_accepted.is_cuda):
+        raise ValueError("out_tokens and num_accepted must be on the GPU")
     size = lib.b200kv_spec_verify_workspace_bytes(seqs, rows, vocab)
     scratch = torch.empty(size, dtype=torch.uint8, device=logits.device)
     status = lib.b200kv_spec_verify(
