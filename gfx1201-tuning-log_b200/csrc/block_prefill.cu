@@ -70,12 +70,29 @@ constexpr int kOffV8 = kOffK + kKStages * kBytes8;
 constexpr int kOffV16 = kOffV8 + kV8Stages * kBytes8;  // [stage][dims 0-63, 64-127][key][128 B]
 constexpr int kSmem = kOffV16 + kV16Stages * 2 * kBytes8;
 
+// A segment, a share's part of an item: what the Q warps leave for the roles that follow
+// them (its reading costs those a few loads; walking the batch there cost them 3300
+// cycles a segment, of instructions that were never in the caches).
+struct Segment {
+  int n, off;               // its tiles, of the item's
+  KeyTiles keys;
+  int kv_end, row0, qlen, t0, kh;
+  int whole, opens, owner;  // holds the item; holds its first tile, and then the share with its last
+  int last;                 // of the share
+  struct {
+    int first, last;        // positions of its first and last query; last < first where it has none
+    int lo, hi, sinks;      // the key tiles that its queries see: below sinks, or lo .. hi
+    __device__ __forceinline__ bool skips(int t) const { return t > hi || (t < lo && t >= sinks); }
+  } q[2];                   // a query tile
+};
+
 struct Shared {
   uint64_t k_full[kKStages], k_empty[kKStages];
   uint64_t v8_full[kV8Stages], v8_empty[kV8Stages], v16_full[kV16Stages], v16_empty[kV16Stages];
   uint64_t q_full[2], q_free[2];                     // [segment parity]
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [query tile][tile parity]
   uint32_t tmem;
+  Segment seg[2];                                    // [segment parity]
   float factor[2][2][kRows];                         // [segment parity][query tile] score factors
   alignas(16) float4 scale[kScales][kMaxPages];    // ks, log2 vs, 1 / vs
   int first[4];                                      // of this share: sequence, head of the CTA's, pair, tile
@@ -118,18 +135,6 @@ __device__ __forceinline__ Pair pair_of(const BlockAttnParams& p, const Seq& s, 
   r.keys = key_tiles<kShift>(p, s.q0 + r.t0, min(s.kv_end, s.q0 + min(s.qlen, r.t0 + 2 * r.tokens)));
   return r;
 }
-// The key tiles of a pair that a query of tile X sees.
-struct Cut {
-  int lo, hi, sinks;
-  __device__ __forceinline__ Cut(const BlockAttnParams& p, const Pair& r, int X) {
-    const int first = r.first(X), last = r.last(X);
-    hi = last < first ? -1 : min(last, r.kv_end - 1) >> kShift;
-    lo = p.window > 0 ? max(0, first - p.window + 1) >> kShift : 0;
-    sinks = (p.sinks + kTile - 1) >> kShift;
-  }
-  __device__ __forceinline__ bool skips(int t) const { return t > hi || (t < lo && t >= sinks); }
-};
-
 // A CTA's share, segment by segment.
 struct Walk {
   const BlockAttnParams& p;
@@ -454,14 +459,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t d_v = tc::sdesc_sw128(smem_u32(smem + kOffV16), kBytes8, 1024);
       const uint32_t t_s = tbase + X * kRows, t_o = tbase + 2 * kRows + X * kRows;
       bool failed = false;
-      int i0 = 0, qk = 0, pv = 0, seg = 0;  // qk, pv: products of this query tile so far
+      int i0 = 0, qk = 0, pv = 0;  // qk, pv: products of this query tile so far
 #pragma unroll 1
-      for (Walk w(p, S, begin, count); w.left > 0; w.next(), ++seg) {
-        const int n = w.count(), off = w.off;
-        const KeyTiles keys = w.r.keys;
-        const Cut cut(p, w.r, X);
+      for (int seg = 0;; ++seg) {
+        if (!mbar_wait_parked(&S.q_full[seg & 1], (seg >> 1) & 1)) break;
+        const Segment& g = S.seg[seg & 1];
+        const int n = g.n, off = g.off;
+        const KeyTiles keys = g.keys;
+        const auto cut = g.q[X];
+        const bool last = g.last;
         const uint64_t d_q = tc::sdesc_sw128(smem_u32(smem + kOffQ + (4 * (seg & 1) + 2 * X) * kBytesQ), 16, 1024);
-        if (!failed) failed = !mbar_wait_parked(&S.q_full[seg & 1], (seg >> 1) & 1);
         bool first = true;
         int jq = 0, jp = 0;  // the tiles whose products with Q, with P come next
 #pragma unroll 1
@@ -513,6 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++pv;
           ++jp;
         }
+        if (last || failed) break;
         mbar_arrive(&S.q_free[seg & 1]);
         i0 += n;
       }
@@ -551,13 +559,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     // A power-of-two prescale a row (maximum in [2^7, 2^8)) with the sign of sm_scale, two
     // terms; eight lanes a row.
     const int qt = tid - kQWarp * 32, c = qt & 7;
-    bool failed = false;
     int seg = 0;
 #pragma unroll 1
     for (Walk w(p, S, begin, count); w.left > 0; w.next(), ++seg) {
       const int b = seg & 1, kh = w.kh();
       const Pair& r = w.r;
-      if (seg >= 2 && !failed) failed = !mbar_wait_parked(&S.q_free[b], ((seg >> 1) - 1) & 1);
+      if (seg >= 2 && !mbar_wait_parked(&S.q_free[b], ((seg >> 1) - 1) & 1)) break;
+      if (qt < 2) {
+        Segment& g = S.seg[b];
+        const int first = r.first(qt), last = r.last(qt);
+        g.q[qt].first = first;
+        g.q[qt].last = last;
+        g.q[qt].hi = last < first ? -1 : min(last, r.kv_end - 1) >> kShift;
+        g.q[qt].lo = p.window > 0 ? max(0, first - p.window + 1) >> kShift : 0;
+        g.q[qt].sinks = (p.sinks + kTile - 1) >> kShift;
+        if (qt == 0) {
+          g.n = w.count();
+          g.off = w.off;
+          g.keys = r.keys;
+          g.kv_end = r.kv_end;
+          g.row0 = r.row0;
+          g.qlen = r.qlen;
+          g.t0 = r.t0;
+          g.kh = kh;
+          g.whole = g.n == r.keys.count;
+          g.opens = w.off == 0;
+          g.owner = g.whole ? share : share_owner(w.item + r.keys.count - 1, total, shares);
+          g.last = w.left <= g.n;
+        }
+      }
       uint4 n0, n1;  // the next row's chunk, in flight
       auto load = [&](int a) {
         const int X = a / kRows, row = a % kRows, tok = over_group(row, inv_group), t = r.t0 + X * r.tokens + tok;
@@ -611,31 +641,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t t_o = tbase + 2 * kRows + X * kRows + lane_off;
     bool failed = false;
-    int i = 0, done = 0, seg = 0;  // done: tiles of this query tile so far
+    const int tokens = kRows / p.group, tok = over_group(row, inv_group);
+    int i = 0, done = 0;  // done: tiles of this query tile so far
 #pragma unroll 1
-    for (Walk w(p, S, begin, count); w.left > 0; w.next(), ++seg) {
-      const int n = w.count(), kh = w.kh(), off = w.off;
-      const int64_t item = w.item;
-      const Pair& r = w.r;
-      const Cut cut(p, r, X);
-      const int tok = over_group(row, inv_group), t = r.t0 + X * r.tokens + tok;
-      const bool valid = tok < r.tokens && t < r.qlen;
-      const int pos = valid ? r.q0 + t : r.last(X);
-      if (!failed) failed = !mbar_wait_parked(&S.q_full[seg & 1], (seg >> 1) & 1);
+    for (int seg = 0;; ++seg) {
+      if (!mbar_wait_parked(&S.q_full[seg & 1], (seg >> 1) & 1)) break;
+      const Segment& g = S.seg[seg & 1];
+      const int n = g.n, off = g.off, kv_end = g.kv_end;
+      const KeyTiles keys = g.keys;
+      const auto cut = g.q[X];
+      const bool valid = tok < tokens && g.t0 + X * tokens + tok < g.qlen;
+      const int pos = valid ? cut.first + tok : cut.last;
       const float coef = S.factor[seg & 1][X][row];
 
       float ref = kNone, l = 0.f;
       bool first = true;
 #pragma unroll 1
       for (int j = 0; j < n; ++j, ++i) {
-        const int tile = r.keys.tile(off + j), key0 = tile * kTile;
+        const int tile = keys.tile(off + j), key0 = tile * kTile;
         if (cut.skips(tile)) continue;
         const int b = done & 1;
         const uint32_t t_s = tbase + X * kRows + b * kTile + lane_off;  // its scores, and its P over them
         if (!failed) failed = !mbar_wait_parked(&S.s_full[X][b], (done >> 1) & 1);
         tc::fence_after_sync();
-        const bool open = key0 + kTile - 1 <= r.first(X) && key0 + kTile <= r.kv_end &&
-                          (p.window == 0 || key0 > r.last(X) - p.window || key0 + kTile <= p.sinks);
+        const bool open = key0 + kTile - 1 <= cut.first && key0 + kTile <= kv_end &&
+                          (p.window == 0 || key0 > cut.last - p.window || key0 + kTile <= p.sinks);
         if (!open) {
           // a tile that some row sees in part: hidden scores become -inf first, so that the
           // loops below stay short (the roles' loops have to fit the instruction caches
@@ -644,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int c = 0; c < kTile / 16; ++c) {
             const int key = key0 + 16 * c;
-            uint32_t m = below(min(pos + 1, r.kv_end) - key);
+            uint32_t m = below(min(pos + 1, kv_end) - key);
             if (p.window > 0) m &= ~below(pos - p.window + 1 - key) | below(p.sinks - key);
             float y[16];
             tc::ld_wait(t_s + 16 * c, y);
@@ -727,53 +757,69 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 
       // ---- the segment's end ----------------------------------------------------------------
-      const bool whole = n == r.keys.count;
-      float* part = p.partials + (int64_t)(2 * blockIdx.x + (item >= begin ? 1 : 0)) * kPartialFloats;
       if (!first && !failed) failed = !mbar_wait_parked(&S.pv_done[X][(done - 1) & 1], ((done - 1) >> 1) & 1);
       tc::fence_after_sync();
-      const float f = whole ? (l > 0.f ? __fdividef(256.f, l) : 0.f) : 256.f;  // V entered as 2^-8 V
-      __nv_bfloat16* dst =
-          p.out + (int64_t)(r.row0 + (valid ? t : 0)) * p.o_st + (int64_t)(kh * p.group + row - tok * p.group) * p.o_sh;
-      float* pdst = part + (X * kRows + row) * kHead;
+      if (g.whole) {
+        // Rows to memory through this query tile's Q, which its products have read: a warp's
+        // 32 rows of 256 bytes, 16-byte chunks swizzled by the row (a thread's own row straight
+        // to memory, 32 lines a store, took 9000 cycles a segment).
+        uint8_t* stage = smem + kOffQ + (4 * (seg & 1) + 2 * X) * kBytesQ + (warp & 3) * 8192;
+        const float f = l > 0.f ? __fdividef(256.f, l) : 0.f;  // V entered as 2^-8 V
 #pragma unroll 1
-      for (int c = 0; c < 8; ++c) {
-        float o[16];
-        if (!first) {
-          tc::ld_wait(t_o + 16 * c, o);
-        } else {
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          tc::ld32_wait(t_o + 32 * c, o);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = 0.f;
-        }
-#pragma unroll
-        for (int k = 0; k < 16; ++k) o[k] *= f;
-        if (valid && whole) {
-#pragma unroll
-          for (int k = 0; k < 16; k += 8) {
+          for (int k = 0; k < 32; k += 8) {
             uint32_t u[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __nv_bfloat162 b = __floats2bfloat162_rn(o[k + 2 * e], o[k + 2 * e + 1]);
-              u[e] = *reinterpret_cast<const uint32_t*>(&b);
+            for (int e = 0; e < 4; ++e) {  // nothing was multiplied into O where the row has no tile
+              const float a = first ? 0.f : o[k + 2 * e] * f, b = first ? 0.f : o[k + 2 * e + 1] * f;
+              const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+              u[e] = *reinterpret_cast<const uint32_t*>(&h);
             }
-            *reinterpret_cast<uint4*>(dst + 16 * c + k) = make_uint4(u[0], u[1], u[2], u[3]);
+            *reinterpret_cast<uint4*>(stage + lane * 256 + (((4 * c + k / 8) ^ (lane & 15)) << 4)) =
+                make_uint4(u[0], u[1], u[2], u[3]);
           }
-        } else if (valid) {
+        }
+        const int64_t at = valid ? (int64_t)(g.row0 + g.t0 + X * tokens + tok) * p.o_st +
+                                       (int64_t)(g.kh * p.group + row - tok * p.group) * p.o_sh
+                                 : -1;
+        __syncwarp();
+#pragma unroll 1
+        for (int k = 0; k < 16; ++k) {
+          const int from = 2 * k + (lane >> 4);
+          const int64_t to = __shfl_sync(0xffffffffu, at, from);
+          const uint4 v =
+              *reinterpret_cast<const uint4*>(stage + from * 256 + (((lane & 15) ^ (from & 15)) << 4));
+          if (to >= 0) *reinterpret_cast<uint4*>(p.out + to + 8 * (lane & 15)) = v;
+        }
+      } else {
+        // o, four columns of all rows side by side, then m and l
+        float* part = p.partials + (int64_t)(2 * blockIdx.x + g.opens) * kPartialFloats;
+#pragma unroll 1
+        for (int c = 0; c < 8; ++c) {
+          float o[16];
+          tc::ld_wait(t_o + 16 * c, o);
 #pragma unroll
           for (int k = 0; k < 16; k += 4)
-            *reinterpret_cast<float4*>(pdst + 16 * c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            if (valid)
+              *reinterpret_cast<float4*>(part + ((4 * c + k / 4) * kPairRows + X * kRows + row) * 4) =
+                  first ? make_float4(0.f, 0.f, 0.f, 0.f)
+                        : make_float4(256.f * o[k], 256.f * o[k + 1], 256.f * o[k + 2], 256.f * o[k + 3]);
+        }
+        if (valid) *reinterpret_cast<float2*>(part + kPairRows * kHead + 2 * (X * kRows + row)) = make_float2(ref, l);
+        if (g.opens && tid == 0) {  // the item begins here and is cut: what its join needs
+          int* rec = p.records + blockIdx.x * 8;
+          rec[1] = g.row0;
+          rec[2] = g.qlen;
+          rec[3] = g.t0;
+          rec[4] = g.kh;
+          rec[5] = g.owner;
+          rec[0] = 1;
         }
       }
-      if (!whole && valid)
-        *reinterpret_cast<float2*>(part + kPairRows * kHead + 2 * (X * kRows + row)) = make_float2(ref, l);
-      if (!whole && item >= begin && tid == 0) {  // the item begins here and is cut: what its join needs
-        int* rec = p.records + blockIdx.x * 8;
-        rec[1] = r.row0;
-        rec[2] = r.qlen;
-        rec[3] = r.t0;
-        rec[4] = kh;
-        rec[5] = share_owner(item + r.keys.count - 1, total, shares);
-        rec[0] = 1;
-      }
+      if (g.last || failed) break;
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&S.q_free[seg & 1]);
@@ -795,7 +841,7 @@ __global__ void __launch_bounds__(128) block_prefill_join_kernel(const BlockAttn
   const int row0 = rec[1], qlen = rec[2], t0 = rec[3], kh = rec[4], c_hi = rec[5];
   const int slot = blockIdx.x % p.slots, c_lo = blockIdx.x / p.slots, tokens = kRows / p.group;
   for (int e = threadIdx.x; e < kJoinRows * (kHead / 4); e += 128) {
-    const int a = blockIdx.y * kJoinRows + e / (kHead / 4), c = e % (kHead / 4);
+    const int a = blockIdx.y * kJoinRows + e % kJoinRows, c = e / kJoinRows;  // row, four columns
     const int X = a / kRows, row = a % kRows, t = t0 + X * tokens + row / p.group;
     if (row >= tokens * p.group || t >= qlen) continue;
     float top = kNone, sum = 0.f;
@@ -814,7 +860,7 @@ __global__ void __launch_bounds__(128) block_prefill_join_kernel(const BlockAttn
           const int64_t cta = (int64_t)(c0 + u) * p.slots + slot;
           const float* q = p.partials + (2 * cta + (c0 + u == c_lo ? 1 : 0)) * kPartialFloats;
           ml[u] = __ldcg(reinterpret_cast<const float2*>(q + kPairRows * kHead + 2 * a));
-          v[u] = __ldcg(reinterpret_cast<const float4*>(q + a * kHead + 4 * c));
+          v[u] = __ldcg(reinterpret_cast<const float4*>(q + (c * kPairRows + a) * 4));
         }
       }
 #pragma unroll
