@@ -57,6 +57,7 @@ constexpr int kMaxPages = 4;
 constexpr int kSoftWarps = 8, kConvWarp = 8, kConvWarps = 2, kQWarp = 10, kQWarps = 6, kMmaWarp = 16;
 constexpr int kTmaWarp = 18, kScaleWarp = 19;
 constexpr int kThreads = 640;
+constexpr int kItemTiles = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;             // m moves when a maximum passes it by 2^8 (P stays within f16)
 constexpr float kMinScale = 8.2718061e-25f, kMaxScale = 1.2089258e24f;  // 2^-80, 2^80
@@ -96,7 +97,8 @@ struct Shared {
   float factor[2][2][kRows];                         // [segment parity][query tile] score factors
   alignas(16) float4 scale[kScales][kMaxPages];    // ks, log2 vs, 1 / vs
   int first[4];                                      // of this share: sequence, head of the CTA's, pair, tile
-  int warp_sum[kThreads / 32];
+  int tiles;                                         // of this share, once it is known to end
+  int2 warp_sum[kThreads / 32];
 };
 
 // Two query tiles of a sequence and the key tiles they see.
@@ -135,30 +137,38 @@ __device__ __forceinline__ Pair pair_of(const BlockAttnParams& p, const Seq& s, 
   r.keys = key_tiles<kShift>(p, s.q0 + r.t0, min(s.kv_end, s.q0 + min(s.qlen, r.t0 + 2 * r.tokens)));
   return r;
 }
-// A CTA's share, segment by segment.
+// A CTA's share, segment by segment, in tiles and `head` more before each item's (what an
+// item costs beside its tiles).
 struct Walk {
   const BlockAttnParams& p;
   Seq s;
   Pair r;
-  int seq, sub, pair, off;
+  int seq, sub, pair, at, head;  // at: in the item
   int left;
   int64_t item;
-  __device__ Walk(const BlockAttnParams& p_, const Shared& S, int64_t begin, int count) : p(p_), left(count) {
+  __device__ Walk(const BlockAttnParams& p_, const Shared& S, int64_t begin, int count, int head_)
+      : p(p_), head(head_), left(count) {
     seq = S.first[0];
     sub = S.first[1];
     pair = S.first[2];
-    off = S.first[3];
-    item = begin - off;
+    at = S.first[3];
+    item = begin - at;
     s = seq_of(p, seq);
     r = pair_of(p, s, pair);
   }
-  __device__ __forceinline__ int count() const { return min(r.keys.count - off, left); }
+  __device__ __forceinline__ int size() const { return r.keys.count + head; }
+  __device__ __forceinline__ int off() const { return max(0, at - head); }
+  __device__ __forceinline__ int count() const { return min(size(), at + left) - head - off(); }
+  __device__ __forceinline__ bool last() const { return left - (size() - at) <= head; }  // no tile after this segment
   __device__ __forceinline__ int kh() const { return blockIdx.x % p.slots * p.heads + sub; }
   __device__ __forceinline__ void next() {
-    left -= count();
-    if (left <= 0) return;
-    item += r.keys.count;
-    off = 0;
+    if (last()) {
+      left = 0;
+      return;
+    }
+    left -= size() - at;
+    item += size();
+    at = 0;
 #pragma unroll 1
     do {
       if (++pair >= s.pairs) {
@@ -269,50 +279,73 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbar_init();
   }
   if (warp == kMmaWarp) tc::tmem_alloc(&S.tmem, 512);
+  if (tid == 0) S.tiles = 0x7fffffff;
   griddep_wait();  // lengths, tables and q may be the previous kernel's
 
   // ---- this CTA's share ----------------------------------------------------------------
   const int per = (p.num_seqs + kThreads - 1) / kThreads;
   const int s_lo = min(p.num_seqs, tid * per), s_hi = min(p.num_seqs, s_lo + per);
-  auto seq_tiles = [&](int seq) {
+  auto seq_tiles = [&](int seq) {  // tiles, items
     const Seq s = seq_of(p, seq);
-    int n = 0;
+    int2 n = make_int2(0, 0);
 #pragma unroll 1
-    for (int i = 0; i < s.pairs; ++i) n += pair_of(p, s, i).keys.count;
+    for (int i = 0; i < s.pairs; ++i) {
+      const int c = pair_of(p, s, i).keys.count;
+      n.x += c;
+      n.y += c > 0;
+    }
     return n;
   };
-  int mine = 0;
+  int2 mine = make_int2(0, 0);
 #pragma unroll 1
-  for (int s = s_lo; s < s_hi; ++s) mine += seq_tiles(s);
-  int incl = mine;
+  for (int s = s_lo; s < s_hi; ++s) {
+    const int2 n = seq_tiles(s);
+    mine.x += n.x;
+    mine.y += n.y;
+  }
+  int2 incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
+    const int x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
+    if (lane >= o) {
+      incl.x += x;
+      incl.y += y;
+    }
   }
   if (lane == 31) S.warp_sum[warp] = incl;
   if (tid == 0) p.records[blockIdx.x * 8] = 0;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  int before = 0, tiles = 0;
+  int2 before = make_int2(0, 0), all = make_int2(0, 0);
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += S.warp_sum[w];
-    tiles += S.warp_sum[w];
+    const int2 v = S.warp_sum[w];
+    if (w < warp) {
+      before.x += v.x;
+      before.y += v.y;
+    }
+    all.x += v.x;
+    all.y += v.y;
   }
-  const int64_t total = (int64_t)tiles * p.heads;
+  const int64_t tiles = (int64_t)all.x * p.heads;
   const int share = blockIdx.x / p.slots;
-  const int64_t shares = min((int64_t)(gridDim.x / p.slots), total);
+  const int64_t shares = min((int64_t)(gridDim.x / p.slots), tiles);
+  // A segment's fixed cost is that of about kItemTiles tiles; where shares are short the
+  // items are cut many times, and a share that held an item's head alone would be empty.
+  const int head = shares > 0 ? (int)min((int64_t)kItemTiles, tiles / shares / 8) : 0;
+  const int64_t total = tiles + (int64_t)all.y * p.heads * head;
   const bool busy = share < shares;
   const int64_t begin = busy ? share_begin(share, total, shares) : 0;
   const int count = busy ? (int)(share_begin(share + 1, total, shares) - begin) : 0;
   if (busy) {
-    int at = before + incl - mine;
-    if (begin >= (int64_t)at * p.heads && begin < (int64_t)(at + mine) * p.heads)
+    const int size = mine.x + mine.y * head;
+    int at = before.x + incl.x + (before.y + incl.y) * head - size;
+    if (begin >= (int64_t)at * p.heads && begin < (int64_t)(at + size) * p.heads)
 #pragma unroll 1
       for (int s = s_lo; s < s_hi; ++s) {
-        const int n = seq_tiles(s);
+        const int2 t = seq_tiles(s);
+        const int n = t.x + t.y * head;
         if (begin < (int64_t)(at + n) * p.heads) {
           int rel = (int)(begin - (int64_t)at * p.heads);
           const Seq q = seq_of(p, s);
@@ -321,7 +354,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           rel %= n;
           int pair = 0;
 #pragma unroll 1
-          for (int m; rel >= (m = pair_of(p, q, pair).keys.count); ++pair) rel -= m;
+          for (;; ++pair) {
+            const int c = pair_of(p, q, pair).keys.count, m = c > 0 ? c + head : 0;
+            if (rel < m) break;
+            rel -= m;
+          }
           S.first[2] = pair;
           S.first[3] = rel;
           break;
@@ -362,10 +399,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     int i = 0;
     bool ok = true;
 #pragma unroll 1
-    for (Walk w(p, S, begin, count); w.left > 0 && ok; w.next()) {
-      const int n = w.count(), kh = w.kh(), kv_end = w.r.kv_end;
+    for (Walk w(p, S, begin, count, head); w.left > 0 && ok; w.next()) {
+      const int n = w.count(), off = w.off(), kh = w.kh(), kv_end = w.r.kv_end;
       const int32_t* row = p.bt + (int64_t)w.seq * p.bt_stride;
-      auto key_of = [&](int j0) { return w.r.keys.tile(w.off + j0 + lane / ppt) * kTile + lane % ppt * bs; };
+      auto key_of = [&](int j0) { return w.r.keys.tile(off + j0 + lane / ppt) * kTile + lane % ppt * bs; };
       auto entry = [&](int j0) {
         if (j0 + lane / ppt >= n) return -1;
         const int key = key_of(j0);
@@ -379,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           cur = nxt;
           nxt = entry(j + tpw);
         }
-        const int key0 = w.r.keys.tile(w.off + j) * kTile;
+        const int key0 = w.r.keys.tile(off + j) * kTile;
         const int boxes = (min(kTile, kv_end - key0) + bs - 1) / bs;
         const int box = lane - j0 * ppt;
         const bool mine = box >= 0 && box < boxes;
@@ -407,11 +444,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_4d(smem + kOffV8 + vs * kBytes8 + box * bs * kHead, &vmap, 0, kh, slot0, cur, &S.v8_full[vs]);
       }
     }
-    if (lane == 0) {  // every copy issued has landed before the CTA may exit
+    if (lane == 0) {
+      // every copy issued has landed before the CTA may exit
 #pragma unroll 1
       for (int j = max(0, i - kKStages); j < i; ++j) mbar_wait_parked(&S.k_full[j % kKStages], (j / kKStages) & 1);
 #pragma unroll 1
       for (int j = max(0, i - kV8Stages); j < i; ++j) mbar_wait_parked(&S.v8_full[j % kV8Stages], (j / kV8Stages) & 1);
+      // the warps that convert V learn that tile i does not come
+      if (ok && i >= kV8Stages) ok = mbar_wait_parked(&S.v8_empty[i % kV8Stages], (i / kV8Stages - 1) & 1);
+      S.tiles = i;
+      if (ok) mbar_arrive(&S.v8_full[i % kV8Stages]);
     }
     __syncwarp();
   } else if (warp == kScaleWarp) {
@@ -420,12 +462,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     int i = 0;
     bool failed = false;
 #pragma unroll 1
-    for (Walk w(p, S, begin, count); w.left > 0; w.next()) {
-      const int n = w.count(), kh = w.kh();
+    for (Walk w(p, S, begin, count, head); w.left > 0; w.next()) {
+      const int n = w.count(), off = w.off(), kh = w.kh();
       const int32_t* row = p.bt + (int64_t)w.seq * p.bt_stride;
       auto load = [&](int j) {  // this lane's block of tile j
         float2 v = make_float2(0.f, 0.f);
-        const int key = j < n && lane < ppt ? w.r.keys.tile(w.off + j) * kTile + (lane << sub) : w.r.kv_end;
+        const int key = j < n && lane < ppt ? w.r.keys.tile(off + j) * kTile + (lane << sub) : w.r.kv_end;
         if (key < w.r.kv_end) {
           const int blk = __ldg(row + (key >> p.shift));
           if (blk >= 0 && blk < p.num_blocks)  // else the block reads as zeros
@@ -531,9 +573,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int ct = tid - kConvWarp * 32, c = ct & 7;  // 16 codes, dims 16 c .., of every 4 kConvWarps-th key
     bool failed = false;
 #pragma unroll 1
-    for (int i = 0; i < count; ++i) {
+    for (int i = 0;; ++i) {
       const int s8 = i % kV8Stages, st = i % kV16Stages;
-      if (!failed) failed = !mbar_wait_parked(&S.v8_full[s8], (i / kV8Stages) & 1);
+      if (failed || !mbar_wait_parked(&S.v8_full[s8], (i / kV8Stages) & 1) || i >= S.tiles) break;
       if (i >= kV16Stages && !failed) failed = !mbar_wait_parked(&S.v16_empty[st], (i / kV16Stages - 1) & 1);
       const uint8_t* src = smem + kOffV8 + s8 * kBytes8;
       uint8_t* dst = smem + kOffV16 + st * 2 * kBytes8 + (c >> 2) * kBytes8;
@@ -561,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int qt = tid - kQWarp * 32, c = qt & 7;
     int seg = 0;
 #pragma unroll 1
-    for (Walk w(p, S, begin, count); w.left > 0; w.next(), ++seg) {
+    for (Walk w(p, S, begin, count, head); w.left > 0; w.next(), ++seg) {
       const int b = seg & 1, kh = w.kh();
       const Pair& r = w.r;
       if (seg >= 2 && !mbar_wait_parked(&S.q_free[b], ((seg >> 1) - 1) & 1)) break;
@@ -575,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         g.q[qt].sinks = (p.sinks + kTile - 1) >> kShift;
         if (qt == 0) {
           g.n = w.count();
-          g.off = w.off;
+          g.off = w.off();
           g.keys = r.keys;
           g.kv_end = r.kv_end;
           g.row0 = r.row0;
@@ -583,9 +625,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           g.t0 = r.t0;
           g.kh = kh;
           g.whole = g.n == r.keys.count;
-          g.opens = w.off == 0;
-          g.owner = g.whole ? share : share_owner(w.item + r.keys.count - 1, total, shares);
-          g.last = w.left <= g.n;
+          g.opens = g.off == 0;
+          g.owner = g.whole ? share : share_owner(w.item + w.size() - 1, total, shares);
+          g.last = w.last();
         }
       }
       uint4 n0, n1;  // the next row's chunk, in flight
