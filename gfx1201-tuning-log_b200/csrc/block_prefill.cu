@@ -234,11 +234,13 @@ __device__ __forceinline__ uint64_t exp2_2(uint64_t x) {
   unpair2(x, a, b);
   return pair2(ex2(a), ex2(b));
 }
-// two e4m3 codes (bytes 2 s, 2 s + 1 of w) -> f16x2 of 2^-8 their values
+// two e4m3 codes (bytes 2 S, 2 S + 1 of w) -> f16x2; codes of NaN become 448
 template <int S>
 __device__ __forceinline__ uint32_t half2_of(uint32_t w) {
-  const uint32_t t = __byte_perm(w, 0u, S ? 0x3424 : 0x1404);  // codes in the high bytes
-  return (t & 0x80008000u) | ((t & 0x7F007F00u) >> 1);
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)(S ? w >> 16 : w & 0xFFFFu)));
+  asm("min.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x5F005F00u));
+  return r;
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -630,23 +632,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           g.last = w.last();
         }
       }
-      uint4 n0, n1;  // the next row's chunk, in flight
-      auto load = [&](int a) {
+      // The rows land where their terms will be (a row's first 64 elements in hi's place, the
+      // others in lo's), all in flight at once, and are laid out in place.
+      auto place = [&](int a) { return smem + kOffQ + (4 * b + 2 * (a / kRows)) * kBytesQ; };
+#pragma unroll 1
+      for (int a = qt / 8; a < 2 * kRows; a += 4 * kQWarps) {
         const int X = a / kRows, row = a % kRows, tok = over_group(row, inv_group), t = r.t0 + X * r.tokens + tok;
-        n0 = n1 = make_uint4(0, 0, 0, 0);
-        if (a < 2 * kRows && tok < r.tokens && t < r.qlen) {
-          const uint4* src = reinterpret_cast<const uint4*>(
-              p.q + (int64_t)(r.row0 + t) * p.q_st + (int64_t)(kh * p.group + row - tok * p.group) * p.q_sh + 16 * c);
-          n0 = __ldg(src);
-          n1 = __ldg(src + 1);
-        }
-      };
-      load(qt / 8);
+        const bool real = tok < r.tokens && t < r.qlen;
+        const __nv_bfloat16* src = p.q + (int64_t)(r.row0 + (real ? t : 0)) * p.q_st +
+                                   (int64_t)(kh * p.group + (real ? row - tok * p.group : 0)) * p.q_sh + 16 * c;
+        const uint32_t dst = smem_u32(place(a) + (c >> 2) * kBytesQ);
+        cp_async16(dst + swz(row, 2 * (c & 3)), src, real ? 16 : 0);
+        cp_async16(dst + swz(row, 2 * (c & 3) + 1), src + 8, real ? 16 : 0);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      __syncwarp();
 #pragma unroll 1
       for (int a = qt / 8; a < 2 * kRows; a += 4 * kQWarps) {
         const int X = a / kRows, row = a % kRows;
+        uint8_t* q = place(a);
+        const uint8_t* raw = q + (c >> 2) * kBytesQ;
+        const uint4 n0 = *reinterpret_cast<const uint4*>(raw + swz(row, 2 * (c & 3)));
+        const uint4 n1 = *reinterpret_cast<const uint4*>(raw + swz(row, 2 * (c & 3) + 1));
         const uint32_t w[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
-        load(a + 4 * kQWarps);
         uint32_t top = max_abs_bf2(max_abs_bf2(max_abs_bf2(w[0], w[1]), max_abs_bf2(w[2], w[3])),
                                    max_abs_bf2(max_abs_bf2(w[4], w[5]), max_abs_bf2(w[6], w[7])));
 #pragma unroll
@@ -667,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           hi[k / 2] = k & 1 ? hi[k / 2] | ch << 16 : ch;
           lo[k / 2] = k & 1 ? lo[k / 2] | cl << 16 : cl;
         }
-        uint8_t* q = smem + kOffQ + (4 * b + 2 * X) * kBytesQ;
+        __syncwarp();  // the row has been read
         *reinterpret_cast<uint4*>(q + swz(row, c)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4*>(q + kBytesQ + swz(row, c)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         if (c == 0)
@@ -806,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // 32 rows of 256 bytes, 16-byte chunks swizzled by the row (a thread's own row straight
         // to memory, 32 lines a store, took 9000 cycles a segment).
         uint8_t* stage = smem + kOffQ + (4 * (seg & 1) + 2 * X) * kBytesQ + (warp & 3) * 8192;
-        const float f = l > 0.f ? __fdividef(256.f, l) : 0.f;  // V entered as 2^-8 V
+        const float f = l > 0.f ? __fdividef(1.f, l) : 0.f;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float o[32];
@@ -847,8 +856,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 16; k += 4)
             if (valid)
               *reinterpret_cast<float4*>(part + ((4 * c + k / 4) * kPairRows + X * kRows + row) * 4) =
-                  first ? make_float4(0.f, 0.f, 0.f, 0.f)
-                        : make_float4(256.f * o[k], 256.f * o[k + 1], 256.f * o[k + 2], 256.f * o[k + 3]);
+                  first ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
         if (valid) *reinterpret_cast<float2*>(part + kPairRows * kHead + 2 * (X * kRows + row)) = make_float2(ref, l);
         if (g.opens && tid == 0) {  // the item begins here and is cut: what its join needs
