@@ -54,9 +54,9 @@ constexpr int kBytes8 = kTile * kHead;   // K or V codes of a tile, and half the
 constexpr int kKStages = 3, kV8Stages = 2, kV16Stages = 3;
 constexpr int kScales = 8;               // tiles whose blocks' scales are held: see the scale warp
 constexpr int kMaxPages = 4;
-constexpr int kSoftWarps = 8, kConvWarp = 8, kConvWarps = 2, kQWarp = 10, kQWarps = 6, kMmaWarp = 16;
-constexpr int kTmaWarp = 18, kScaleWarp = 19;
-constexpr int kThreads = 640;
+constexpr int kSoftWarps = 8, kConvWarp = 8, kConvWarps = 2, kQWarp = 10, kQWarps = 4, kMmaWarp = 14;
+constexpr int kTmaWarp = 16, kScaleWarp = 17;
+constexpr int kThreads = 576;
 constexpr int kItemTiles = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;             // m moves when a maximum passes it by 2^8 (P stays within f16)
@@ -70,6 +70,11 @@ constexpr int kOffK = kOffQ + 8 * kBytesQ;
 constexpr int kOffV8 = kOffK + kKStages * kBytes8;
 constexpr int kOffV16 = kOffV8 + kV8Stages * kBytes8;  // [stage][dims 0-63, 64-127][key][128 B]
 constexpr int kSmem = kOffV16 + kV16Stages * 2 * kBytes8;
+
+// A sequence: its first row of q, query tokens, first query's position, keys, pairs of query tiles.
+struct Seq {
+  int row0, qlen, q0, kv_end, pairs;
+};
 
 // A segment, a share's part of an item: what the Q warps leave for the roles that follow
 // them (its reading costs those a few loads; walking the batch there cost them 3300
@@ -96,7 +101,8 @@ struct Shared {
   Segment seg[2];                                    // [segment parity]
   float factor[2][2][kRows];                         // [segment parity][query tile] score factors
   alignas(16) float4 scale[kScales][kMaxPages];    // ks, log2 vs, 1 / vs
-  int first[4];                                      // of this share: sequence, head of the CTA's, pair, tile
+  int first[4];                                      // of this share: sequence, head of the CTA's, pair, place in it
+  Seq start;                                         // and that sequence
   int tiles;                                         // of this share, once it is known to end
   int2 warp_sum[kThreads / 32];
 };
@@ -110,9 +116,6 @@ struct Pair {
   // positions of the first and last query of tile X; last < first where it is empty
   __device__ __forceinline__ int first(int X) const { return q0 + t0 + X * tokens; }
   __device__ __forceinline__ int last(int X) const { return q0 + min(qlen, t0 + (X + 1) * tokens) - 1; }
-};
-struct Seq {
-  int row0, qlen, q0, kv_end, pairs;
 };
 __device__ __forceinline__ Seq seq_of(const BlockAttnParams& p, int seq) {
   Seq s;
@@ -153,7 +156,7 @@ struct Walk {
     pair = S.first[2];
     at = S.first[3];
     item = begin - at;
-    s = seq_of(p, seq);
+    s = S.start;
     r = pair_of(p, s, pair);
   }
   __device__ __forceinline__ int size() const { return r.keys.count + head; }
@@ -285,26 +288,41 @@ __global__ void __launch_bounds__(kThreads, 1)
   griddep_wait();  // lengths, tables and q may be the previous kernel's
 
   // ---- this CTA's share ----------------------------------------------------------------
-  const int per = (p.num_seqs + kThreads - 1) / kThreads;
-  const int s_lo = min(p.num_seqs, tid * per), s_hi = min(p.num_seqs, s_lo + per);
-  auto seq_tiles = [&](int seq) {  // tiles, items
-    const Seq s = seq_of(p, seq);
+  // Sequences are counted by a warp each, a lane a pair, and neighbours by different warps
+  // (a thread a sequence spent up to 33000 cycles on two prompts of 8192 tokens).
+  auto tiles_of = [&](const Seq& s) {  // tiles, items
     int2 n = make_int2(0, 0);
 #pragma unroll 1
-    for (int i = 0; i < s.pairs; ++i) {
+    for (int i = lane; i < s.pairs; i += 32) {
       const int c = pair_of(p, s, i).keys.count;
       n.x += c;
       n.y += c > 0;
     }
-    return n;
+    return make_int2(__reduce_add_sync(0xffffffffu, n.x), __reduce_add_sync(0xffffffffu, n.y));
   };
-  int2 mine = make_int2(0, 0);
+  const int per = (p.num_seqs + kThreads - 1) / kThreads;  // sequences of a bin
+  int2* bins = reinterpret_cast<int2*>(smem);              // [kThreads], before Q is there
+  {
+    const int bin = lane * (kThreads / 32) + warp;
+    int2 mine = make_int2(0, 0);
 #pragma unroll 1
-  for (int s = s_lo; s < s_hi; ++s) {
-    const int2 n = seq_tiles(s);
-    mine.x += n.x;
-    mine.y += n.y;
+    for (int k = 0; k < per; ++k) {
+      const int seq = bin * per + k;
+      Seq s = {0, 0, 0, 0, 0};
+      if (seq < p.num_seqs) s = seq_of(p, seq);
+#pragma unroll 1
+      for (unsigned many = __ballot_sync(0xffffffffu, s.pairs > 0); many; many &= many - 1) {
+        const int from = __ffs(many) - 1;
+        const Seq g = {0, __shfl_sync(0xffffffffu, s.qlen, from), __shfl_sync(0xffffffffu, s.q0, from),
+                       __shfl_sync(0xffffffffu, s.kv_end, from), __shfl_sync(0xffffffffu, s.pairs, from)};
+        const int2 n = tiles_of(g);
+        if (lane == from) mine = make_int2(mine.x + n.x, mine.y + n.y);
+      }
+    }
+    bins[bin] = mine;
   }
+  __syncthreads();
+  const int2 mine = bins[tid];
   int2 incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -343,30 +361,47 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (busy) {
     const int size = mine.x + mine.y * head;
     int at = before.x + incl.x + (before.y + incl.y) * head - size;
-    if (begin >= (int64_t)at * p.heads && begin < (int64_t)(at + size) * p.heads)
+    const unsigned here = __ballot_sync(
+        0xffffffffu, begin >= (int64_t)at * p.heads && begin < (int64_t)(at + size) * p.heads);
+    if (here) {  // the warp that has the share's first tile
+      at = __shfl_sync(0xffffffffu, at, __ffs(here) - 1);
 #pragma unroll 1
-      for (int s = s_lo; s < s_hi; ++s) {
-        const int2 t = seq_tiles(s);
+      for (int seq = (warp * 32 + __ffs(here) - 1) * per; seq < p.num_seqs; ++seq) {
+        const Seq s = seq_of(p, seq);
+        const int2 t = tiles_of(s);
         const int n = t.x + t.y * head;
-        if (begin < (int64_t)(at + n) * p.heads) {
-          int rel = (int)(begin - (int64_t)at * p.heads);
-          const Seq q = seq_of(p, s);
-          S.first[0] = s;
-          S.first[1] = rel / n;
-          rel %= n;
-          int pair = 0;
-#pragma unroll 1
-          for (;; ++pair) {
-            const int c = pair_of(p, q, pair).keys.count, m = c > 0 ? c + head : 0;
-            if (rel < m) break;
-            rel -= m;
-          }
-          S.first[2] = pair;
-          S.first[3] = rel;
-          break;
+        if (begin >= (int64_t)(at + n) * p.heads) {
+          at += n;
+          continue;
         }
-        at += n;
+        int rel = (int)(begin - (int64_t)at * p.heads);
+        const int sub = rel / n;
+        rel -= sub * n;
+#pragma unroll 1
+        for (int i = lane; i - lane < s.pairs; i += 32) {
+          const int c = i < s.pairs ? pair_of(p, s, i).keys.count : 0, m = c > 0 ? c + head : 0;
+          int upto = m;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+          }
+          const unsigned past = __ballot_sync(0xffffffffu, rel < upto);
+          if (past) {
+            if (lane == __ffs(past) - 1) {
+              S.start = s;
+              S.first[0] = seq;
+              S.first[1] = sub;
+              S.first[2] = i;
+              S.first[3] = rel - (upto - m);
+            }
+            break;
+          }
+          rel -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+        break;
       }
+    }
   }
   __syncthreads();
   const int inv_group = (65536 + p.group - 1) / p.group;
@@ -634,53 +669,64 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // The rows land where their terms will be (a row's first 64 elements in hi's place, the
       // others in lo's), all in flight at once, and are laid out in place.
-      auto place = [&](int a) { return smem + kOffQ + (4 * b + 2 * (a / kRows)) * kBytesQ; };
+      auto place = [&](int X) { return smem + kOffQ + (4 * b + 2 * X) * kBytesQ; };
 #pragma unroll 1
-      for (int a = qt / 8; a < 2 * kRows; a += 4 * kQWarps) {
-        const int X = a / kRows, row = a % kRows, tok = over_group(row, inv_group), t = r.t0 + X * r.tokens + tok;
-        const bool real = tok < r.tokens && t < r.qlen;
-        const __nv_bfloat16* src = p.q + (int64_t)(r.row0 + (real ? t : 0)) * p.q_st +
-                                   (int64_t)(kh * p.group + (real ? row - tok * p.group : 0)) * p.q_sh + 16 * c;
-        const uint32_t dst = smem_u32(place(a) + (c >> 2) * kBytesQ);
-        cp_async16(dst + swz(row, 2 * (c & 3)), src, real ? 16 : 0);
-        cp_async16(dst + swz(row, 2 * (c & 3) + 1), src + 8, real ? 16 : 0);
+      for (int a = qt / 8; a < kRows; a += 4 * kQWarps) {
+        const int tok = over_group(a, inv_group);
+#pragma unroll
+        for (int X = 0; X < 2; ++X) {
+          const int t = r.t0 + X * r.tokens + tok;
+          const bool real = tok < r.tokens && t < r.qlen;
+          const __nv_bfloat16* src = p.q + (int64_t)(r.row0 + (real ? t : 0)) * p.q_st +
+                                     (int64_t)(kh * p.group + (real ? a - tok * p.group : 0)) * p.q_sh + 16 * c;
+          const uint32_t dst = smem_u32(place(X) + (c >> 2) * kBytesQ);
+          cp_async16(dst + swz(a, 2 * (c & 3)), src, real ? 16 : 0);
+          cp_async16(dst + swz(a, 2 * (c & 3) + 1), src + 8, real ? 16 : 0);
+        }
       }
       cp_async_commit();
       cp_async_wait<0>();
       __syncwarp();
+      // two rows at a time, each a long chain of dependent operations
 #pragma unroll 1
-      for (int a = qt / 8; a < 2 * kRows; a += 4 * kQWarps) {
-        const int X = a / kRows, row = a % kRows;
-        uint8_t* q = place(a);
-        const uint8_t* raw = q + (c >> 2) * kBytesQ;
-        const uint4 n0 = *reinterpret_cast<const uint4*>(raw + swz(row, 2 * (c & 3)));
-        const uint4 n1 = *reinterpret_cast<const uint4*>(raw + swz(row, 2 * (c & 3) + 1));
-        const uint32_t w[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
-        uint32_t top = max_abs_bf2(max_abs_bf2(max_abs_bf2(w[0], w[1]), max_abs_bf2(w[2], w[3])),
-                                   max_abs_bf2(max_abs_bf2(w[4], w[5]), max_abs_bf2(w[6], w[7])));
+      for (int a = qt / 8; a < kRows; a += 4 * kQWarps) {
+        uint32_t hi[2][4], lo[2][4];
+        float factor[2];
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) top = max_abs_bf2(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const uint32_t mx = max(top & 0x7FFFu, top >> 16 & 0x7FFFu);  // bits of the row's largest magnitude
-        const int E = (int)(mx >> 7);
-        int sh = (E == 0xFF || mx == 0) ? 0 : 134 - E;
-        sh = max(-126, min(126, sh));
-        const float up = __uint_as_float((uint32_t)(sh + 127) << 23 | (p.sm_scale < 0.f ? 0x80000000u : 0u));
-        // hi: the magnitude rounded to 4 significant bits (half away from zero); the rest has
-        // at most 5 and is exact in bf16
-        uint32_t hi[4], lo[4];
+        for (int X = 0; X < 2; ++X) {
+          const uint8_t* raw = place(X) + (c >> 2) * kBytesQ;
+          const uint4 n0 = *reinterpret_cast<const uint4*>(raw + swz(a, 2 * (c & 3)));
+          const uint4 n1 = *reinterpret_cast<const uint4*>(raw + swz(a, 2 * (c & 3) + 1));
+          const uint32_t w[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+          uint32_t top = max_abs_bf2(max_abs_bf2(max_abs_bf2(w[0], w[1]), max_abs_bf2(w[2], w[3])),
+                                     max_abs_bf2(max_abs_bf2(w[4], w[5]), max_abs_bf2(w[6], w[7])));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t x = (w[k] + 0x00080008u) & 0xFFF0FFF0u, y = sub_bf2(w[k], x);
-          const uint32_t ch = e4m3x2(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xFFFF0000u) * up);
-          const uint32_t cl = e4m3x2(__uint_as_float(y << 16) * up, __uint_as_float(y & 0xFFFF0000u) * up);
-          hi[k / 2] = k & 1 ? hi[k / 2] | ch << 16 : ch;
-          lo[k / 2] = k & 1 ? lo[k / 2] | cl << 16 : cl;
+          for (int o = 1; o < 8; o <<= 1) top = max_abs_bf2(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const uint32_t mx = max(top & 0x7FFFu, top >> 16 & 0x7FFFu);  // bits of the row's largest magnitude
+          const int E = (int)(mx >> 7);
+          int sh = (E == 0xFF || mx == 0) ? 0 : 134 - E;
+          sh = max(-126, min(126, sh));
+          const float up = __uint_as_float((uint32_t)(sh + 127) << 23 | (p.sm_scale < 0.f ? 0x80000000u : 0u));
+          // hi: the magnitude rounded to 4 significant bits (half away from zero); the rest has
+          // at most 5 and is exact in bf16
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t x = (w[k] + 0x00080008u) & 0xFFF0FFF0u, y = sub_bf2(w[k], x);
+            const uint32_t ch = e4m3x2(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xFFFF0000u) * up);
+            const uint32_t cl = e4m3x2(__uint_as_float(y << 16) * up, __uint_as_float(y & 0xFFFF0000u) * up);
+            hi[X][k / 2] = k & 1 ? hi[X][k / 2] | ch << 16 : ch;
+            lo[X][k / 2] = k & 1 ? lo[X][k / 2] | cl << 16 : cl;
+          }
+          factor[X] = fabsf(p.sm_scale) * kLog2e * __uint_as_float((uint32_t)(127 - sh) << 23);
         }
-        __syncwarp();  // the row has been read
-        *reinterpret_cast<uint4*>(q + swz(row, c)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(q + kBytesQ + swz(row, c)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if (c == 0)
-          S.factor[b][X][row] = fabsf(p.sm_scale) * kLog2e * __uint_as_float((uint32_t)(127 - sh) << 23);
+        __syncwarp();  // the rows have been read
+#pragma unroll
+        for (int X = 0; X < 2; ++X) {
+          uint8_t* q = place(X);
+          *reinterpret_cast<uint4*>(q + swz(a, c)) = make_uint4(hi[X][0], hi[X][1], hi[X][2], hi[X][3]);
+          *reinterpret_cast<uint4*>(q + kBytesQ + swz(a, c)) = make_uint4(lo[X][0], lo[X][1], lo[X][2], lo[X][3]);
+          if (c == 0) S.factor[b][X][a] = factor[X];
+        }
       }
       tc::fence_proxy_async_smem();
       __syncwarp();
