@@ -3,14 +3,13 @@
 // rows per kv head.
 //
 // A CTA holds two 128-row query tiles (tokens x the heads of one kv head) and walks
-// 128-key tiles, each read once for both:
+// 64-key tiles, each read once for both:
 //   S = Q K^T   kind::f8f6f4, Q as two e4m3 terms (8 significant bits), K as stored;
 //   O += P V    kind::f16, P from tensor memory, V converted to f16 in shared memory.
 // Splitting P into two e4m3 terms instead keeps V as stored but costs the softmax
-// threads five operations a score; converting V costs four warps four operations a
-// code, a quarter as many codes as scores, and P keeps f16's 11 bits.  An e4m3 code's
-// bits shifted by one are the f16 of 2^-8 its value, subnormals included (codes of
-// NaN become 480: no non-finite value enters the product).
+// threads five operations a score; converting V costs two warps two operations a pair
+// of codes, a quarter as many codes as scores, and P keeps f16's 11 bits.  e4m3 is
+// exact in f16; codes of NaN become 448, so that no hidden key's V reaches a row.
 //
 // Block scales ks, vs as in block_decode.cu: x = sm_scale log2(e) ks (q . k) + log2(vs),
 // P = 2^(x - m), and the softmax sum adds P / vs.  A softmax thread is a query row:
@@ -20,16 +19,25 @@
 // for the product.
 //
 // Shares of the batch's tiles as in block_decode.cu, an item being the two query
-// tiles of a kv head; what a cut item's shares leave is joined by a second kernel.
+// tiles of a kv head, which counts kItemTiles tiles more than it has (with none, the
+// shares of many short items ended last: four prompts of 512 to 2048 tokens 143 ->
+// 121 us); what a cut item's shares leave is joined by a second kernel.
 //
 // Tiles are 64 keys, so that tensor memory holds two score tiles of each query tile
 // (4 x 64 columns) beside the two outputs (2 x 128): while the softmax works on one,
 // the next is multiplied, and P V and the Q K^T that reuses its columns leave the
 // softmax's chain.  Shared memory then has room for the next item's Q as well.
 //
-// Roles: 8 softmax warps (four a query tile, a thread a row), 2 that convert V, 6 that
-// lay out Q (with 2, prompts of 2048 tokens and less waited for it: 243 -> 162 us), a warp a query tile that issues its products, a TMA warp, a warp for the
-// blocks' scales.
+// Roles: 8 softmax warps (four a query tile, a thread a row), 2 that convert V, 4 that
+// lay out Q and describe the segments (with 2, eight prompts of 2048 tokens 442 -> 456
+// us), a warp a query tile that issues its products, a TMA warp, a warp for the blocks'
+// scales.
+//
+// Two prompts of 8192 tokens (32 heads over 8): 1395 us, 788 TFLOP/s, 47 % of the bf16
+// peak; eight of 2048: 442 us, 622.  A tile takes 2500 cycles: the softmax warps' chain
+// (maxima 560, P 1450, waiting for scores 330) beside 800 of issuing products; neither
+// the exponentials alone nor the products alone change the time when left out.
+// Instructions are few on purpose: unrolling the loop over P made it 4 % slower.
 
 #include <cuda.h>
 #include <cuda_bf16.h>

@@ -16,7 +16,9 @@
 // resident at once, and their barriers leave the memory idle).
 //
 // Statistics are fp32; the temperature divides as a multiplication by its
-// reciprocal.  Streaming the logits bounds a full batch (320 rows of 128256: 164 MB).
+// reciprocal.  Streaming the logits bounds a full batch (64 sequences, 226 MB with the
+// drafts' distributions and the noise: 50 us, 4.6 TB/s, 70 % of the copy rate); one
+// sequence (10 us) is two launches, each a chain of loads, reduction and join.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
