@@ -79,6 +79,16 @@ __device__ __forceinline__ KeyTiles key_tiles(const BlockAttnParams& p, int firs
   return t;
 }
 
+// Tiles that an item counts beside its own, for what each costs at its ends: `most`,
+// fewer where shares are short, as items are cut more often than they end there, and a
+// share that held no more than an item's head would be empty.
+__device__ __forceinline__ int item_head(int64_t tiles, int shares, int most) {
+  int head = 0;
+#pragma unroll 1
+  while (head < most && tiles >= (int64_t)3 * (head + 1) * shares) ++head;
+  return shares > 0 ? head : 0;
+}
+
 // Share i of `shares` begins at tile i total / shares; the owner of a tile is the
 // last share that does not begin past it.
 __device__ __forceinline__ int64_t share_begin(int64_t share, int64_t total, int64_t shares) {

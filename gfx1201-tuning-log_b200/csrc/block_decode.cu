@@ -71,6 +71,8 @@ constexpr float kMaxScale = 1.2089258e24f;  // 2^80
 constexpr float kMasked = -3e38f;           // the score of a key that a query does not see
 constexpr float kNone = -1e30f;             // the reference of a row that has seen no key
 
+constexpr int kItemTiles = 4;               // what a segment's end costs in tiles (24 rows)
+
 template <int R>
 struct Shape {
   // rows of a softmax thread; warps of a group: four quadrants of 32 keys for each
@@ -116,7 +118,7 @@ struct Shared {
   alignas(16) float alpha[2][R];                     // and what its last move scales O and l by
   alignas(16) float fin_m[2][R], fin_l[2][4][R];
   int first_seq, first_prefix, last;
-  int warp_sum[Shape<R>::kWarps];
+  int2 warp_sum[Shape<R>::kWarps];
 };
 
 // CH per-row values from shared memory (16-byte aligned)
@@ -168,28 +170,33 @@ __device__ __forceinline__ Span span_of(const BlockAttnParams& p, int seq, int m
 }
 
 // A CTA's share, segment by segment (a segment: consecutive tiles of one item, an
-// item: a sequence and kv head).
+// item: a sequence and kv head), in tiles and `head` more before each item's.
 struct Walk {
   const BlockAttnParams& p;
   int max_rows;
   Span s;
-  int seq, sub, off, left;  // sub: which of the CTA's p.heads kv heads
-  int64_t item;  // index of the item's first tile in the slot's order
-  __device__ Walk(const BlockAttnParams& p_, int max_rows_, int seq_, int prefix, int64_t begin, int count)
-      : p(p_), max_rows(max_rows_), seq(seq_), left(count) {
+  int seq, sub, at, head, left;  // sub: which of the CTA's p.heads kv heads; at: in the item
+  int64_t item;  // where the item begins in the slot's order
+  __device__ Walk(const BlockAttnParams& p_, int max_rows_, int seq_, int prefix, int64_t begin, int count, int head_)
+      : p(p_), max_rows(max_rows_), seq(seq_), head(head_), left(count) {
     s = span_of(p, seq, max_rows);
     const int rel = (int)(begin - (int64_t)prefix * p.heads);
-    sub = rel / s.keys.count;
-    off = rel - sub * s.keys.count;
-    item = begin - off;
+    sub = rel / size();
+    at = rel - sub * size();
+    item = begin - at;
   }
-  __device__ __forceinline__ int count() const { return min(s.keys.count - off, left); }
+  __device__ __forceinline__ int size() const { return s.keys.count + head; }
+  __device__ __forceinline__ int off() const { return max(0, at - head); }
+  __device__ __forceinline__ int count() const { return min(size(), at + left) - head - off(); }
   __device__ __forceinline__ int kh() const { return blockIdx.x % p.slots * p.heads + sub; }
   __device__ __forceinline__ void next() {
-    left -= count();
-    if (left <= 0) return;
-    item += s.keys.count;
-    off = 0;
+    left -= size() - at;
+    if (left <= head) {  // no tile after this segment
+      left = 0;
+      return;
+    }
+    item += size();
+    at = 0;
     if (++sub == p.heads) {
       sub = 0;
 #pragma unroll 1
@@ -237,37 +244,52 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
   // ---- this CTA's share: an inclusive scan of the sequences' tile counts -------------
   const int per = (p.num_seqs + kThreads - 1) / kThreads;
   const int s_lo = min(p.num_seqs, tid * per), s_hi = min(p.num_seqs, s_lo + per);
-  int mine = 0;
+  int2 mine = make_int2(0, 0);  // tiles, sequences that have some
 #pragma unroll 1
-  for (int s = s_lo; s < s_hi; ++s) mine += span_of(p, s, R).keys.count;
-  int incl = mine;
+  for (int s = s_lo; s < s_hi; ++s) {
+    const int n = span_of(p, s, R).keys.count;
+    mine.x += n;
+    mine.y += n > 0;
+  }
+  int2 incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
+    const int x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
+    if (lane >= o) {
+      incl.x += x;
+      incl.y += y;
+    }
   }
   if (lane == 31) S.warp_sum[warp] = incl;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  int before = 0, tiles = 0;
+  int2 before = make_int2(0, 0), all = make_int2(0, 0);
 #pragma unroll
   for (int w = 0; w < SH::kWarps; ++w) {
-    if (w < warp) before += S.warp_sum[w];
-    tiles += S.warp_sum[w];
+    const int2 v = S.warp_sum[w];
+    if (w < warp) {
+      before.x += v.x;
+      before.y += v.y;
+    }
+    all.x += v.x;
+    all.y += v.y;
   }
-  const int64_t total = (int64_t)tiles * p.heads;
+  const int64_t tiles = (int64_t)all.x * p.heads;
   const int slot = blockIdx.x % p.slots, share = blockIdx.x / p.slots;
-  const int64_t shares = min((int64_t)(gridDim.x / p.slots), total);
+  const int64_t shares = min((int64_t)(gridDim.x / p.slots), tiles);
+  const int head = item_head(tiles, (int)shares, kItemTiles);
+  const int64_t total = tiles + (int64_t)all.y * p.heads * head;
   const bool busy = share < shares;
   const int64_t begin = busy ? share_begin(share, total, shares) : 0;
   const int count = busy ? (int)(share_begin(share + 1, total, shares) - begin) : 0;
   if (busy) {
-    int at = before + incl - mine;  // tiles of the sequences before this thread's
-    if (begin >= (int64_t)at * p.heads && begin < (int64_t)(at + mine) * p.heads)
+    const int size = mine.x + mine.y * head;
+    int at = before.x + incl.x + (before.y + incl.y) * head - size;  // the sequences before this thread's
+    if (begin >= (int64_t)at * p.heads && begin < (int64_t)(at + size) * p.heads)
 #pragma unroll 1
       for (int s = s_lo; s < s_hi; ++s) {
-        const int n = span_of(p, s, R).keys.count;
+        const int c = span_of(p, s, R).keys.count, n = c > 0 ? c + head : 0;
         if (begin < (int64_t)(at + n) * p.heads) {
           S.first_seq = s;
           S.first_prefix = at;
@@ -305,13 +327,13 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
     int i = 0;
     bool ok = true;
 #pragma unroll 1
-    for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0 && ok; w.next()) {
-      const int n = w.count(), kh = w.kh();
+    for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count, head); w.left > 0 && ok; w.next()) {
+      const int n = w.count(), off = w.off(), kh = w.kh();
       const int32_t* row = p.bt + (int64_t)w.seq * p.bt_stride;
       auto entry = [&](int j0) {  // block of this lane's page of tiles j0 ..
         const int j = j0 + lane / ppt;
         if (j >= n) return -1;
-        const int page = w.s.keys.tile(w.off + j) * ppt + lane % ppt;
+        const int page = w.s.keys.tile(off + j) * ppt + lane % ppt;
         return page << p.shift < w.s.kv_end ? __ldg(row + page) : -1;
       };
       int cur = entry(0), nxt = entry(tpw);
@@ -328,7 +350,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
           ok = false;
           break;
         }
-        const int keys = min(kTile, w.s.kv_end - w.s.keys.tile(w.off + j) * kTile);
+        const int keys = min(kTile, w.s.kv_end - w.s.keys.tile(off + j) * kTile);
         const int pages = (keys + bs - 1) >> p.shift;
         if (lane == 0) mbar_arrive_expect_tx(&S.kv_full[st], (uint32_t)(pages * bs * kHead));
         __syncwarp();
@@ -354,7 +376,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
       bool failed = false;
       int i = 0, seg = 0;
 #pragma unroll 1
-      for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0; w.next(), ++seg) {
+      for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count, head); w.left > 0; w.next(), ++seg) {
         if (!failed) failed = !mbar_wait_parked(&S.q_full[seg & 1], (seg >> 1) & 1);
 #pragma unroll 1
         for (int j = w.count(); j > 0; --j, ++i) {
@@ -381,7 +403,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
       bool failed = false;
       int i = 0;
 #pragma unroll 1
-      for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count); w.left > 0; w.next()) {
+      for (Walk w(p, R, S.first_seq, S.first_prefix, begin, count, head); w.left > 0; w.next()) {
         const int n = w.count();
 #pragma unroll 1
         for (int j = 0; j < n; ++j, ++i) {
@@ -461,14 +483,14 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&S.q_full[qb]);
     };
-    Walk w(p, R, S.first_seq, S.first_prefix, begin, count);
+    Walk w(p, R, S.first_seq, S.first_prefix, begin, count, head);
     put_q(w.s, w.kh(), 0);
 #pragma unroll 1
     for (; w.left > 0; ++seg) {
       const int n = w.count(), qb = seg & 1, kh = w.kh();
       const Span s = w.s;
       const int64_t item = w.item;
-      const int off = w.off, rows = s.qlen * p.group;
+      const int off = w.off(), rows = s.qlen * p.group;
       // the next segment's Q goes out now, so that its first product need not wait for
       // this one's end (the buffer's last reader ended with the segment before)
       w.next();
@@ -636,7 +658,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
             make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
       };
       const bool whole = n == s.keys.count;
-      float* part_o = p.partials + (int64_t)(2 * blockIdx.x + (item >= begin ? 1 : 0)) * kPartialFloats;
+      float* part_o = p.partials + (int64_t)(2 * blockIdx.x + (off == 0 ? 1 : 0)) * kPartialFloats;
 #pragma unroll 1
       for (int e = tid; e < rows * (kHead / 4); e += kSoftThreads) {
         const int a = e / (kHead / 4), c = e % (kHead / 4);
@@ -656,7 +678,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
       }
       if (!whole) {
         named_bar_sync(kAll, kSoftThreads);
-        const int c_lo = share_owner(item, total, shares), c_hi = share_owner(item + s.keys.count - 1, total, shares);
+        const int c_lo = share_owner(item + head, total, shares), c_hi = share_owner(item + head + s.keys.count - 1, total, shares);
         if (tid == 0) {
           int* counter = p.counters + c_lo * p.slots + slot;  // one item at most is cut at a share's end
           __threadfence();  // the other threads' partials, which the barrier has ordered before this
@@ -668,8 +690,6 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
         if (S.last) {
           // the shares of the item in order, kJoin loads of each kind in flight
           constexpr int kJoin = R <= 16 ? 8 : 4;
-          // later shares begin inside the item: it is their first
-          const int at0 = item >= share_begin(c_lo, total, shares) ? 1 : 0;
 #pragma unroll 1
           for (int e = tid; e < rows * (kHead / 4); e += kSoftThreads) {
             const int a = e / (kHead / 4), c = e % (kHead / 4);
@@ -686,7 +706,7 @@ __global__ void __launch_bounds__(Shape<R>::kThreads, 1)
                 v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (c0 + u <= c_hi) {
                   const int64_t cta = (int64_t)(c0 + u) * p.slots + slot;
-                  const float* q = p.partials + (2 * cta + (c0 + u == c_lo ? at0 : 0)) * kPartialFloats;
+                  const float* q = p.partials + (2 * cta + (c0 + u == c_lo ? 1 : 0)) * kPartialFloats;
                   ml[u] = __ldcg(reinterpret_cast<const float2*>(q + kMaxRows * kHead + 2 * a));
                   v[u] = __ldcg(reinterpret_cast<const float4*>(q + a * kHead + 4 * c));
                 }

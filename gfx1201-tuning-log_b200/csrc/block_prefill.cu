@@ -359,9 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t tiles = (int64_t)all.x * p.heads;
   const int share = blockIdx.x / p.slots;
   const int64_t shares = min((int64_t)(gridDim.x / p.slots), tiles);
-  // A segment's fixed cost is that of about kItemTiles tiles; where shares are short the
-  // items are cut many times, and a share that held an item's head alone would be empty.
-  const int head = shares > 0 ? (int)min((int64_t)kItemTiles, tiles / shares / 8) : 0;
+  const int head = item_head(tiles, (int)shares, kItemTiles);
   const int64_t total = tiles + (int64_t)all.y * p.heads * head;
   const bool busy = share < shares;
   const int64_t begin = busy ? share_begin(share, total, shares) : 0;
