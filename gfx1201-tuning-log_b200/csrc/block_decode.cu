@@ -37,7 +37,7 @@
 // stores.  Keys no query sees have their V rows zeroed, so stale or non-finite codes
 // never reach an output.
 //
-// 60 sequences of 2k to 32k tokens (2.1 GB): 341 us, 6.29 TB/s, 96 % of the copy rate;
+// 60 sequences of 2k to 32k tokens (2.1 GB): 338 us, 6.34 TB/s, 97 % of the copy rate;
 // one of 4096 tokens (8.4 MB): 12.0 us, of which 0.7 are its two tiles a CTA and the
 // rest a chain: the share 1.3 us, block table and first pages 1.5, scores 0.9, the
 // segment's end 1.7, the join of its shares 1.7 to 3.8.

@@ -17,7 +17,7 @@
 //
 // Statistics are fp32; the temperature divides as a multiplication by its
 // reciprocal.  Streaming the logits bounds a full batch (64 sequences, 226 MB with the
-// drafts' distributions and the noise: 50 us, 4.6 TB/s, 70 % of the copy rate); one
+// drafts' distributions and the noise: 48 us, 4.7 TB/s, 72 % of the copy rate); one
 // sequence (10 us) is two launches, each a chain of loads, reduction and join.
 
 #include <cuda_bf16.h>
@@ -434,10 +434,12 @@ int spec_verify_launch(const void* logits, int64_t ld, int half, const int64_t* 
   p.accepted = accepted;
   p.vocab = vocab;
   p.num_seqs = num_seqs;
-  p.chunk = chunk_of(num_rows, vocab, 12);
+  // 8 CTAs an SM for the statistics (12: eight sequences 19.2 against 16.3 us), 3 for the
+  // race, whose CTAs each begin with the join (6: 64 sequences 49.8 against 48.0 us)
+  p.chunk = chunk_of(num_rows, vocab, 8);
   p.chunks = cdiv(vocab, p.chunk);
   p.stats = static_cast<float4*>(workspace);
-  p.rchunk = chunk_of(num_seqs, vocab, 6);
+  p.rchunk = chunk_of(num_seqs, vocab, 3);
   p.rchunks = cdiv(vocab, p.rchunk);
   p.races = p.stats + (size_t)num_rows * p.chunks;
   p.counters = reinterpret_cast<int*>(p.races + (size_t)num_seqs * p.rchunks);
