@@ -30,11 +30,11 @@
 //
 // Roles: 8 softmax warps (four a query tile, a thread a row), 2 that convert V, 4 that
 // lay out Q and describe the segments (with 2, eight prompts of 2048 tokens 442 -> 456
-// us), a warp a query tile that issues its products, a TMA warp, a warp for the blocks'
+// us; the softmax warps' help with a share's first changed nothing), a warp a query tile that issues its products, a TMA warp, a warp for the blocks'
 // scales.
 //
-// Two prompts of 8192 tokens (32 heads over 8): 1395 us, 788 TFLOP/s, 47 % of the bf16
-// peak; eight of 2048: 442 us, 622.  A tile takes 2500 cycles: the softmax warps' chain
+// Two prompts of 8192 tokens (32 heads over 8): 1369 us, 803 TFLOP/s, 47 % of the bf16
+// peak; eight of 2048: 434 us, 633.  A tile takes 2500 cycles: the softmax warps' chain
 // (maxima 560, P 1450, waiting for scores 330) beside 800 of issuing products; neither
 // the exponentials alone nor the products alone change the time when left out.
 // Instructions are few on purpose: unrolling the loop over P made it 4 % slower.
