@@ -283,8 +283,8 @@ int block_append_launch(const b200kv_block_cache* c, const void* qkv, int64_t qk
                         const int32_t* lens, int num_tokens, int hq, void* stream) {
   const int bad = block_cache_check(c);
   if (bad != B200KV_OK) return bad;
-  if (!qkv || !cos_sin || !q_out || !cu || !lens || max_pos <= 0 || num_tokens < 0 || hq <= 0 ||
-      hq % c->num_kv_heads)
+  if (!cos_sin || !cu || !lens || max_pos <= 0 || num_tokens < 0 || hq <= 0 || hq % c->num_kv_heads ||
+      (num_tokens > 0 && (!qkv || !q_out)))
     return B200KV_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) |
        reinterpret_cast<uintptr_t>(cos_sin)) & 15)

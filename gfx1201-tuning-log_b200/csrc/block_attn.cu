@@ -48,7 +48,8 @@ size_t block_attn_workspace_bytes(int num_seqs, int num_kv_heads) {
 int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args* a, void* stream) {
   const int bad = block_cache_check(c);
   if (bad != B200KV_OK) return bad;
-  if (!a || !a->q || !a->out || !a->cu_seqlens_q || !a->seq_lens) return B200KV_ERR_INVALID_ARG;
+  if (!a || !a->cu_seqlens_q || !a->seq_lens) return B200KV_ERR_INVALID_ARG;
+  if (a->num_tokens != 0 && (!a->q || !a->out)) return B200KV_ERR_INVALID_ARG;  // no tokens: no rows to point to
   if (a->num_tokens < 0 || a->max_qlen <= 0 || a->max_seq_len < 0 || a->num_q_heads <= 0 || a->window < 0 ||
       a->sinks < 0 || a->num_q_heads % c->num_kv_heads)
     return B200KV_ERR_INVALID_ARG;
@@ -86,6 +87,7 @@ int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args*
   p.window = a->window;
   p.sinks = a->sinks;
   p.hkv = c->num_kv_heads;
+  p.all = 0;
   char* ws = static_cast<char*>(a->workspace);
   p.counters = reinterpret_cast<int*>(ws);
   p.records = reinterpret_cast<int*>(ws + kCounterBytes);
@@ -106,9 +108,12 @@ int block_attn_launch(const b200kv_block_cache* c, const b200kv_block_attn_args*
   if (rows > kMaxRows) {
     CUtensorMap km64 = km, vm64 = vm;
     if (c->block_size > 64 && !maps(&km64, &vm64, 64)) return B200KV_ERR_UNSUPPORTED;
+    // A single sequence that may have many rows is left to that kernel whatever it has: the
+    // other's launch, empty as a rule, costs 3 us (33 tokens at 12000: 39.8 against 36.5 us).
+    p.all = c->num_seqs == 1;
     e = block_prefill_launch(km64, vm64, p, st);
   }
-  if (e == cudaSuccess) e = block_decode_launch(km, vm, p, rows < kMaxRows ? (int)rows : kMaxRows, st);
+  if (e == cudaSuccess && !p.all) e = block_decode_launch(km, vm, p, rows < kMaxRows ? (int)rows : kMaxRows, st);
   return e == cudaSuccess ? B200KV_OK : B200KV_ERR_LAUNCH;
 }
 

@@ -55,6 +55,7 @@ struct BlockAttnParams {
   // The batch's key tiles, ordered by (sequence, kv head, queries, tile), are cut into
   // equal shares; `slots` CTAs walk a share at once, each for `heads` of the kv heads.
   int heads, slots;
+  int all;          // the many-query kernel takes sequences of few rows too
   float* partials;  // two a CTA: what a share leaves of an item that it cuts
   int* counters;    // [kMaxCtas], zero between calls: arrivals at the item cut at a CTA's end
   int* records;     // [kMaxCtas][8]: the many-query kernel's cut items, for the join after it

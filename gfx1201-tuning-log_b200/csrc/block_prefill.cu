@@ -133,7 +133,7 @@ __device__ __forceinline__ Seq seq_of(const BlockAttnParams& p, int seq) {
   s.q0 = total - s.qlen;
   s.kv_end = min(total, p.max_blocks << p.shift);
   const int tokens = kRows / p.group;
-  const bool many = s.qlen > kMaxRows || s.qlen * p.group > kMaxRows;
+  const bool many = s.qlen > kMaxRows || s.qlen * p.group > kMaxRows || (p.all && s.qlen > 0);
   s.pairs = many ? (s.qlen - 1) / (2 * tokens) + 1 : 0;
   return s;
 }

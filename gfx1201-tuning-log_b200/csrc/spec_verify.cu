@@ -409,16 +409,23 @@ int spec_verify_launch(const void* logits, int64_t ld, int half, const int64_t* 
                        const float* uniforms, const float* noise, int64_t noise_ld, const float* temperature,
                        const float* draft, int64_t draft_ld, int64_t* out, int32_t* accepted, int num_seqs,
                        int num_rows, int vocab, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!logits || !tokens || !cu || !uniforms || !noise || !out || !accepted) return B200KV_ERR_INVALID_ARG;
+  if (!cu || (num_seqs > 0 && (!noise || !accepted)) ||
+      (num_rows > 0 && (!logits || !tokens || !uniforms || !out)))
+    return B200KV_ERR_INVALID_ARG;
   if (num_seqs < 0 || num_rows < 0 || vocab <= 0 || ld < vocab || noise_ld < vocab || (draft && draft_ld < vocab))
     return B200KV_ERR_INVALID_ARG;
   if ((int64_t)num_rows * kMaxChunks > 0x7fffffff || (int64_t)num_seqs * kMaxChunks > 0x7fffffff)
     return B200KV_ERR_UNSUPPORTED;
+  if (num_seqs == 0) return B200KV_OK;
   if (!workspace || workspace_bytes < spec_verify_workspace_bytes(num_seqs, num_rows, vocab))
     return B200KV_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return B200KV_ERR_MISALIGNED;
   if (sm_major_current_device() < 10) return B200KV_ERR_NO_DEVICE;
-  if (num_seqs == 0 || num_rows == 0) return B200KV_OK;
+  if (num_rows == 0)  // nobody has a draft
+    return cudaMemsetAsync(accepted, 0, (size_t)num_seqs * sizeof(int32_t), static_cast<cudaStream_t>(stream)) ==
+                   cudaSuccess
+               ? B200KV_OK
+               : B200KV_ERR_LAUNCH;
   VerifyParams p;
   p.logits = logits;
   p.ld = ld;

@@ -477,7 +477,8 @@ int b200kv_block_append(const b200kv_block_cache* cache, const void* qkv, int64_
  * and sees the keys j <= p with window == 0, j > p - window or j < sinks:
  *   out[row, h, :] = sum_j softmax_j(sm_scale q . K[j]) V[j]      (bf16)
  * A query that sees nothing (p < 0) gives zeros.  GQA 1 to 16.
- *   num_tokens    rows of q; max_qlen, max_seq_len  upper bounds over the batch
+ *   num_tokens    rows of q (0: nothing is done, q and out may be null);
+ *                 max_qlen, max_seq_len  upper bounds over the batch
  *   workspace     b200kv_block_attn_workspace_bytes bytes, 256-byte aligned, zeroed
  *                 once before its first use (every call leaves its counters at
  *                 zero); calls that share one are ordered on one stream. */
